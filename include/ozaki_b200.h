@@ -419,6 +419,34 @@ int ozk_selftest_timeout(int budget_ms, int32_t* status_dev, int32_t* ok_dev, vo
  * it; lines not marked persisting may use the set-aside while no persisting
  * data holds it. */
 int ozk_set_l2_persisting(size_t bytes, size_t* previous);
+/* ------------------------------------------------- 16-bit training and serving
+ * Products beside the FP64 path (no counterpart in the reference): low-rank
+ * adapters of many requests on one shared projection, and layer inputs kept as
+ * int8 codes between the forward and the backward pass. */
+
+/* Element types of these entry points. */
+#define OZK_DT_BF16 0
+#define OZK_DT_F16 1
+#define OZK_DT_F32 2
+
+/* Y = X W^T + T B_i^T with T = alpha scale[i] X A_i^T, i = ids[row].
+ *   X [M][K] (ldx), W [N][K] (ldw), A [E][r][K], B [E][N][r], all of type dt
+ *   (OZK_DT_BF16 or OZK_DT_F16); A and B contiguous.
+ *   ids: int32 [M], or NULL (every row belongs to adapter 0); a row whose id is
+ *   outside [0, E) has no adapter.  scale: FP32 [E] or NULL (ones).
+ *   Y [M][N] (ldy) of type dt; low: FP32 [M][r], receives T (0 for rows without
+ *   an adapter), or NULL.
+ * Sums are FP32; T enters the second product as the sum of two 16-bit values
+ * (with OZK_DT_F16, |T| must stay below 65504).  1 <= r <= 128.  Nothing may
+ * alias Y or low.  Operands whose base or row stride is not a multiple of 16
+ * bytes are copied into the workspace first. */
+size_t ozk_matmul_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E);
+int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* A,
+                        const void* B, const int32_t* ids, const float* scale, double alpha,
+                        void* Y, int64_t ldy, float* low, int64_t M, int64_t N, int64_t K, int r,
+                        int E, int dt, void* workspace, size_t ws_bytes, int32_t* status_dev,
+                        void* stream);
+
 /* Library version string. */
 const char* ozk_version(void);
 

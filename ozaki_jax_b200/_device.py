@@ -75,3 +75,23 @@ def to_host_f64(t):
 
 def stream_handle(device):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Here:
+    """No change of device."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device):
+    """Context in which `device` is the current CUDA device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)

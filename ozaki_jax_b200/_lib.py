@@ -31,6 +31,10 @@ OZK_MULTI_NOWAIT = 0x1
 OZK_MULTI_BF16 = 0x2
 OZK_NCCL_ID_BYTES = 128
 
+OZK_DT_BF16 = 0
+OZK_DT_F16 = 1
+OZK_DT_F32 = 2
+
 OZK_ACC_F64 = 0
 OZK_ACC_PRODUCTS = 1
 OZK_ACC_FIXED = 2
@@ -101,6 +105,9 @@ SIGNATURES = {
     "ozk_residual_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int, c_int]),
     "ozk_residual_f64": (c_int, [vp, c_i64, vp, c_i64, vp, c_i64, vp, c_i64, c_i64, c_i64, c_i64,
                                  c_int, c_int, c_int, vp, c_size, vp, vp]),
+    "ozk_matmul_adapters_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int, c_int]),
+    "ozk_matmul_adapters": (c_int, [vp, c_i64, vp, c_i64, vp, vp, vp, vp, c_dbl, vp, c_i64, vp,
+                                    c_i64, c_i64, c_i64, c_int, c_int, c_int, vp, c_size, vp, vp]),
     "ozk_check_status": (c_int, [vp, vp]),
     "ozk_gemm_stats": (c_int, [vp]),
     "ozk_selftest_timeout": (c_int, [c_int, vp, vp, vp]),

@@ -1,0 +1,843 @@
+// Low-rank adapters of many requests beside a shared projection:
+//   T = s_i X A_i^T,  Y = X W^T + T B_i^T,  i = ids[row]
+// and the gradient's first half, which is the same product read the other way:
+//   U = s_i dY B_i,   dX = dY W + U A_i.
+//
+// Both run as two kernels, the second started while the first still runs:
+//   k_low_rank / k_low_rank_rows   T (FP32) and its split T = hi + lo into two
+//                                  16-bit values;
+//   k_linear                       the shared product, with T's columns as
+//                                  further columns of the contraction.
+//
+// The adapters of a tile's rows.  A tile of 128 rows may belong to many
+// adapters.  A TMEM lane of an MMA with M = 128 is a row of the tile, and
+// tcgen05.mma can leave lanes alone: so for each distinct adapter of the tile
+// one MMA chain T B_i^T runs over the whole tile with the lanes of the other
+// rows masked.  No row is moved, no zero is multiplied by another adapter's
+// NaN, and any order of ids is right; contiguous requests cost one or two
+// chains per tile.
+//
+// T between the kernels.  Rounded once to BF16, T would add an error of 2^-9
+// of itself to every output; as hi + lo it carries 16 bits or more (2^-17), at
+// the price of r more columns of the contraction.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "ozk_tile16.cuh"
+
+namespace ozk {
+
+namespace {
+
+constexpr int kRows = 128;       // rows of a tile (TMEM lanes)
+constexpr int kKB = 64;          // contraction elements per stage: 128 bytes
+constexpr int kMaxRank = 128;
+constexpr int kMaxStages = 16;
+constexpr int kThreads = 192;    // producer warp, MMA warp, four epilogue warps
+
+// Columns of the split T of rank r: [hi 32 | lo 32] up to rank 32, else the
+// high parts of ceil(r / 64) blocks of 64, then the low parts.
+__host__ __device__ inline int split_half(int r) { return r <= 32 ? 32 : (r + 63) / 64 * 64; }
+
+struct LinearArgs {
+  const int32_t* ids;
+  void* Y;
+  int64_t ldy;
+  int64_t M;
+  int N, nkb, E, r;
+  int bf16, y_vec;
+  int stages, xrows, tiles_n;
+  int32_t* status;
+  uint64_t budget_ns;
+};
+
+// Ring of shared-memory stages: the index and phase parity of step `it`.
+struct Ring {
+  int n;
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ explicit Ring(int stages) : n(stages) {}
+  __device__ void next() {
+    if (++s == n) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+};
+
+// 8 or 16 consecutive output columns of one row.
+__device__ __forceinline__ void store_cols(void* Y, int64_t at, const uint32_t* v, int n, bool bf16,
+                                           bool vec) {
+  uint16_t* y = (uint16_t*)Y + at;
+  if (vec && n >= 8) {
+    uint4 q;
+    q.x = pack16(bf16, __uint_as_float(v[0]), __uint_as_float(v[1]));
+    q.y = pack16(bf16, __uint_as_float(v[2]), __uint_as_float(v[3]));
+    q.z = pack16(bf16, __uint_as_float(v[4]), __uint_as_float(v[5]));
+    q.w = pack16(bf16, __uint_as_float(v[6]), __uint_as_float(v[7]));
+    *(uint4*)y = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) y[i] = round16(bf16, __uint_as_float(v[i]));
+  }
+}
+
+// Sum over the CTAs of the cluster, in rank order, of the FP32 partial at
+// shared-memory address `a` of each.
+__device__ __forceinline__ float cluster_sum(uint32_t a, int splits) {
+  float s = 0.0f;
+  for (int q = 0; q < splits; ++q) {
+    uint32_t ra;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(q));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ra) : "memory");
+    s += v;
+  }
+  return s;
+}
+
+// ---------------------------------------------------------------- k_linear
+//
+// One CTA per 128 x BN tile, or a cluster of CTAs per tile that split the
+// contraction (and the adapters) between them and add their FP32 partials in
+// rank order through distributed shared memory: deterministic, no scratch.
+// MNB: the shared operand's rows are contraction indexes (W of dX = dY W),
+// read as MN-major tiles.
+template <int BN, bool MNB>
+__global__ void __launch_bounds__(kThreads)
+    k_linear(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW,
+             const __grid_constant__ CUtensorMap mapT, const __grid_constant__ CUtensorMap mapB,
+             const __grid_constant__ LinearArgs g) {
+  constexpr int B_BYTES = BN * 128;
+  constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int a_bytes = g.xrows * 128;
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + g.stages * a_bytes;
+  __shared__ SlotList<4> slots;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, slots_ready;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort_word;
+  volatile int* s_abort = &s_abort_word;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t splits, rank;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+  rank = cluster_ctarank();
+  const int tile = blockIdx.x / splits;
+  const int tm = tile / g.tiles_n, tn = tile - tm * g.tiles_n;
+  const int64_t row0 = (int64_t)tm * kRows;
+  const int col0 = tn * BN;
+  const int kb0 = (int)((int64_t)g.nkb * rank / splits);
+  const int kb1 = (int)((int64_t)g.nkb * (rank + 1) / splits);
+  const int half = split_half(g.r);
+  const int blocks = half < 64 ? 1 : half / 64 * 2;  // stages per adapter
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < g.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&done, 1);
+    mbar_init(&slots_ready, 1);
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&s_tmem, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      Ring rg(g.stages);
+      bool ok = true;
+      int issued = 0;
+      const uint32_t bytes = (uint32_t)(a_bytes + B_BYTES);
+      auto load = [&](const CUtensorMap* ma, int ax, const CUtensorMap* mb, int bx, int bz) {
+        if (!mbar_wait(&empty[rg.s], rg.ph ^ 1, s_abort, g.status, g.budget_ns)) return false;
+        mbar_arrive_expect_tx(&full[rg.s], bytes);
+        tma_load_3d(sA + rg.s * a_bytes, ma, &full[rg.s], ax, (int)row0, 0);
+        uint8_t* b = sB + rg.s * B_BYTES;
+        if constexpr (MNB) {
+#pragma unroll
+          for (int j = 0; j < BN / 64; ++j)
+            tma_load_3d(b + j * 8192, mb, &full[rg.s], col0 + 64 * j, bx, bz);
+        } else {
+          tma_load_3d(b, mb, &full[rg.s], bx, col0, bz);
+        }
+        rg.next();
+        ++issued;
+        return true;
+      };
+      for (int kb = kb0; ok && kb < kb1; ++kb) ok = load(&mapX, kb * kKB, &mapW, kb * kKB, 0);
+      // The split T comes from the kernel before this one.
+      grid_wait();
+      ok = ok && mbar_wait(&slots_ready, 0, s_abort, g.status, g.budget_ns);
+      const int n = ok ? slots.n : 0;
+      for (int j = rank; ok && j < n; j += splits)
+        for (int b = 0; ok && b < blocks; ++b) {
+          // hi and lo blocks of the same ranks in turn, against the same B_i
+          const int ax = blocks == 1 ? 0 : (b & 1) * half + (b >> 1) * 64;
+          ok = load(&mapT, ax, &mapB, blocks == 1 ? 0 : (b >> 1) * 64, slots.id[j]);
+        }
+      // Every copy lands before the shared memory is reused or released.
+      Ring back(g.stages);
+      for (int i = 0; i < issued; ++i, back.next())
+        if (i >= issued - g.stages)
+          mbar_wait(&full[back.s], back.ph, nullptr, g.status, g.budget_ns);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_16(g.bf16, kRows, BN, false, MNB);
+      Ring rg(g.stages);
+      bool ok = true;
+      auto desc_b = [&](uint32_t b0, int kk) {
+        return MNB ? umma_desc_mn128(b0 + kk * 2048, 8192) : umma_desc_sw128(b0 + kk * 32);
+      };
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a0 = smem_u32(sA + rg.s * a_bytes), b0 = smem_u32(sB + rg.s * B_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < kKB / 16; ++kk)
+          umma_bf16(tmem, umma_desc_sw128(a0 + kk * 32), desc_b(b0, kk), idesc,
+                    (kb != kb0) || kk != 0);
+        umma_commit(&empty[rg.s]);
+        rg.next();
+      }
+      ok = ok && mbar_wait(&slots_ready, 0, s_abort, g.status, g.budget_ns);
+      const int n = ok ? slots.n : 0;
+      for (int j = rank; ok && j < n; j += splits) {
+        const uint32_t m0 = slots.off[j][0], m1 = slots.off[j][1], m2 = slots.off[j][2],
+                       m3 = slots.off[j][3];
+        for (int b = 0; b < blocks; ++b) {
+          if (!mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + rg.s * a_bytes), b0 = smem_u32(sB + rg.s * B_BYTES);
+          const int left = g.r - (b >> 1) * 64;
+          const int steps = left >= 64 ? 4 : (left + 15) / 16;
+          for (int kk = 0; kk < steps; ++kk) {
+            umma_16_masked(tmem, umma_desc_sw128(a0 + kk * 32), desc_b(b0, kk), idesc, 1, m0, m1,
+                           m2, m3);
+            if (blocks == 1)
+              umma_16_masked(tmem, umma_desc_sw128(a0 + 64 + kk * 32), desc_b(b0, kk), idesc, 1, m0,
+                             m1, m2, m3);
+          }
+          umma_commit(&empty[rg.s]);
+          rg.next();
+        }
+      }
+      umma_commit(&done);
+      mbar_wait(&done, 0, nullptr, g.status, g.budget_ns);
+    }
+    __syncwarp();
+  } else {
+    if (warp == 2) {
+      if (g.r > 0) build_slots<4>(g.ids, row0, g.M, g.E, &slots, lane);
+      else if (lane == 0) slots.n = 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&slots_ready);
+    }
+    mbar_wait(&done, 0, nullptr, g.status, g.budget_ns);
+  }
+  // The MMAs are done and the copies have landed: the stages are free.
+  __syncthreads();
+  tc_fence_after();
+  const int mrows = g.M - row0 < kRows ? (int)(g.M - row0) : kRows;
+  if (splits == 1) {
+    if (warp >= 2) {
+      const int q = warp & 3;
+      const int64_t row = row0 + q * 32 + lane;
+#pragma unroll
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+        tmem_wait_ld();
+        if (row < g.M)
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            const int n = g.N - (col0 + c + i);
+            if (n > 0) store_cols(g.Y, row * g.ldy + col0 + c + i, v + i, n, g.bf16, g.y_vec);
+          }
+      }
+    }
+  } else {
+    float* part = (float*)smem;  // [row][BN + 1]
+    if (warp >= 2) {
+      const int q = warp & 3;
+      const int r = q * 32 + lane;
+      if (q * 32 < mrows) {
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+          tmem_wait_ld();
+          if (r < mrows)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part[r * (BN + 1) + c + i] = __uint_as_float(v[i]);
+        }
+      }
+    }
+    cluster_sync();
+    const int share = BN / (int)splits;  // a power of two >= 4
+    const int c0 = (int)rank * share;
+    for (int e = threadIdx.x; e < mrows * share; e += kThreads) {
+      const int r = e / share, c = c0 + e - r * share;
+      const float s = cluster_sum(smem_u32(&part[r * (BN + 1) + c]), (int)splits);
+      if (col0 + c < g.N) ((uint16_t*)g.Y)[(row0 + r) * g.ldy + col0 + c] = round16(g.bf16, s);
+    }
+    cluster_sync();  // no CTA leaves while a peer reads its partials
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- low rank
+
+struct LowArgs {
+  const int32_t* ids;
+  const float* scale;
+  float alpha;
+  float* low;        // [M][r] FP32, or NULL
+  uint16_t* split;   // [M][2 half], or NULL
+  int64_t M;
+  int nkb, E, r, rp;  // rp: r rounded up to 16
+  int bf16;
+  int xstages, astages, xrows;
+  int32_t* status;
+  uint64_t budget_ns;
+};
+
+// Rounds t to its high and low 16-bit parts and stores them in the split T.
+__device__ __forceinline__ void store_split(uint16_t* split, int64_t row, int half, int c, float t,
+                                            bool bf16) {
+  const uint16_t hi = round16(bf16, t);
+  float rest = t - widen16(bf16, hi);
+  if (!(fabsf(rest) <= 3.0e38f)) rest = 0.0f;  // t not finite: hi says so by itself
+  split[row * 2 * half + c] = hi;
+  split[row * 2 * half + half + c] = round16(bf16, rest);
+}
+
+// T of a tile of 128 rows: one accumulator of rp columns; each block of 64
+// contraction elements of X is loaded once and multiplied with the same block
+// of every adapter of the tile, each into its own lanes.  The CTAs of a
+// cluster split the contraction.  Bound by reading X.
+template <bool MNB>
+__global__ void __launch_bounds__(kThreads)
+    k_low_rank(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapA,
+               const __grid_constant__ LowArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int x_bytes = g.xrows * 128;
+  const int a_bytes = MNB ? (g.rp + 63) / 64 * 8192 : g.rp * 128;
+  uint8_t* sX = smem;
+  uint8_t* sA = smem + g.xstages * x_bytes;
+  __shared__ SlotList<4> slots;
+  __shared__ uint64_t xfull[kMaxStages], xempty[kMaxStages], afull[kMaxStages], aempty[kMaxStages],
+      done;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort_word;
+  volatile int* s_abort = &s_abort_word;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t splits, rank;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+  rank = cluster_ctarank();
+  const int64_t row0 = (int64_t)(blockIdx.x / splits) * kRows;
+  const int kb0 = (int)((int64_t)g.nkb * rank / splits);
+  const int kb1 = (int)((int64_t)g.nkb * (rank + 1) / splits);
+  uint32_t cols = 32;
+  while (cols < (uint32_t)g.rp) cols *= 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < g.xstages; ++i) {
+      mbar_init(&xfull[i], 1);
+      mbar_init(&xempty[i], 1);
+    }
+    for (int i = 0; i < g.astages; ++i) {
+      mbar_init(&afull[i], 1);
+      mbar_init(&aempty[i], 1);
+    }
+    mbar_init(&done, 1);
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&s_tmem, cols);
+  if (warp == 2) build_slots<4>(g.ids, row0, g.M, g.E, &slots, lane);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_release();  // after the allocation: the next kernel's CTAs cannot take this CTA's TMEM
+  const uint32_t tmem = s_tmem;
+  const int n = slots.n;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      Ring rx(g.xstages), ra(g.astages);
+      bool ok = true;
+      int ix = 0, ia = 0;
+      for (int kb = kb0; ok && kb < kb1; ++kb) {
+        ok = mbar_wait(&xempty[rx.s], rx.ph ^ 1, s_abort, g.status, g.budget_ns);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&xfull[rx.s], (uint32_t)x_bytes);
+        tma_load_3d(sX + rx.s * x_bytes, &mapX, &xfull[rx.s], kb * kKB, (int)row0, 0);
+        rx.next();
+        ++ix;
+        for (int j = 0; j < n; ++j) {
+          ok = mbar_wait(&aempty[ra.s], ra.ph ^ 1, s_abort, g.status, g.budget_ns);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&afull[ra.s], (uint32_t)a_bytes);
+          uint8_t* d = sA + ra.s * a_bytes;
+          if constexpr (MNB) {
+            for (int c = 0; c < g.rp; c += 64)
+              tma_load_3d(d + c * 128, &mapA, &afull[ra.s], c, kb * kKB, slots.id[j]);
+          } else {
+            tma_load_3d(d, &mapA, &afull[ra.s], kb * kKB, 0, slots.id[j]);
+          }
+          ra.next();
+          ++ia;
+        }
+      }
+      Ring bx(g.xstages), ba(g.astages);
+      for (int i = 0; i < ix; ++i, bx.next())
+        if (i >= ix - g.xstages) mbar_wait(&xfull[bx.s], bx.ph, nullptr, g.status, g.budget_ns);
+      for (int i = 0; i < ia; ++i, ba.next())
+        if (i >= ia - g.astages) mbar_wait(&afull[ba.s], ba.ph, nullptr, g.status, g.budget_ns);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_16(g.bf16, kRows, g.rp, false, MNB);
+      Ring rx(g.xstages), ra(g.astages);
+      bool ok = n > 0;
+      for (int kb = kb0; ok && kb < kb1; ++kb) {
+        ok = mbar_wait(&xfull[rx.s], rx.ph, s_abort, g.status, g.budget_ns);
+        if (!ok) break;
+        const uint32_t x0 = smem_u32(sX + rx.s * x_bytes);
+        for (int j = 0; j < n; ++j) {
+          ok = mbar_wait(&afull[ra.s], ra.ph, s_abort, g.status, g.budget_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + ra.s * a_bytes);
+#pragma unroll
+          for (int kk = 0; kk < kKB / 16; ++kk)
+            umma_16_masked(tmem, umma_desc_sw128(x0 + kk * 32),
+                           MNB ? umma_desc_mn128(a0 + kk * 2048, 8192)
+                               : umma_desc_sw128(a0 + kk * 32),
+                           idesc, (kb != kb0) || kk != 0, slots.off[j][0], slots.off[j][1],
+                           slots.off[j][2], slots.off[j][3]);
+          umma_commit(&aempty[ra.s]);
+          ra.next();
+        }
+        if (!ok) break;
+        umma_commit(&xempty[rx.s]);
+        rx.next();
+      }
+      umma_commit(&done);
+      mbar_wait(&done, 0, nullptr, g.status, g.budget_ns);
+    }
+    __syncwarp();
+  } else {
+    mbar_wait(&done, 0, nullptr, g.status, g.budget_ns);
+  }
+  __syncthreads();
+  tc_fence_after();
+  const int mrows = g.M - row0 < kRows ? (int)(g.M - row0) : kRows;
+  const int ldp = g.rp + 1;
+  float* part = (float*)smem;
+  if (warp >= 2) {
+    const int q = warp & 3;
+    const int r = q * 32 + lane;
+    if (q * 32 < mrows)
+      for (int c = 0; c < g.rp; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+        tmem_wait_ld();
+        if (r < mrows)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) part[r * ldp + c + i] = __uint_as_float(v[i]);
+      }
+  }
+  cluster_sync();
+  // Rows of the tile are dealt to the CTAs of the cluster.
+  const int half = split_half(g.r);
+  const int r0 = mrows * (int)rank / (int)splits, r1 = mrows * ((int)rank + 1) / (int)splits;
+  for (int e = threadIdx.x; e < (r1 - r0) * half; e += kThreads) {
+    const int r = r0 + e / half, c = e % half;
+    const int64_t row = row0 + r;
+    float t = 0.0f;
+    const int i = row_adapter(g.ids, row, g.M, g.E);
+    if (i >= 0 && c < g.r)
+      t = cluster_sum(smem_u32(&part[r * ldp + c]), (int)splits) *
+          (g.scale ? g.alpha * g.scale[i] : g.alpha);
+    if (g.low && c < g.r) g.low[row * g.r + c] = t;
+    if (g.split) store_split(g.split, row, half, c, t, g.bf16);
+  }
+  cluster_sync();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, cols);
+  }
+}
+
+// T of few rows (decoding): one CTA per row and four ranks, the contraction
+// split over its threads.  Every row reads its own A_i, so nothing is shared
+// that a matrix instruction could use; bound by the latency of the reads.
+constexpr int kLowThreads = 256;
+constexpr int kLowRanks = 4;
+
+__global__ void __launch_bounds__(kLowThreads)
+    k_low_rank_rows(const uint16_t* X, int64_t ldx, const uint16_t* A, int64_t lda, int64_t K,
+                    LowArgs g) {
+  grid_release();
+  __shared__ float part[kLowThreads / 32][kLowRanks];
+  const int half = split_half(g.r);
+  const int64_t row = blockIdx.x;
+  const int c0 = blockIdx.y * kLowRanks;
+  const int i = row_adapter(g.ids, row, g.M, g.E);
+  float acc[kLowRanks] = {};
+  if (i >= 0 && c0 < g.r) {
+    const uint16_t* x = X + row * ldx;
+    const uint16_t* a[kLowRanks];
+#pragma unroll
+    for (int j = 0; j < kLowRanks; ++j) {
+      const int c = c0 + j < g.r ? c0 + j : g.r - 1;
+      a[j] = A + ((int64_t)i * g.r + c) * lda;
+    }
+    // X's and A's rows start on 16 bytes (padded before this kernel otherwise).
+    const int64_t K8 = K & ~(int64_t)7;
+#pragma unroll 2
+    for (int64_t k = threadIdx.x * 8; k < K8; k += kLowThreads * 8) {
+      const uint4 xv = *(const uint4*)(x + k);
+      uint4 av[kLowRanks];
+#pragma unroll
+      for (int j = 0; j < kLowRanks; ++j) av[j] = __ldg((const uint4*)(a[j] + k));
+      const uint32_t* xw = (const uint32_t*)&xv;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float x0 = widen16(g.bf16, (uint16_t)xw[w]), x1 = widen16(g.bf16, xw[w] >> 16);
+#pragma unroll
+        for (int j = 0; j < kLowRanks; ++j) {
+          const uint32_t u = ((const uint32_t*)&av[j])[w];
+          acc[j] = fmaf(x0, widen16(g.bf16, (uint16_t)u), acc[j]);
+          acc[j] = fmaf(x1, widen16(g.bf16, u >> 16), acc[j]);
+        }
+      }
+    }
+    const int64_t k = K8 + threadIdx.x;
+    if (k < K) {
+      const float xv = widen16(g.bf16, x[k]);
+#pragma unroll
+      for (int j = 0; j < kLowRanks; ++j) acc[j] = fmaf(xv, widen16(g.bf16, a[j][k]), acc[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kLowRanks; ++j)
+    for (int o = 16; o; o >>= 1) acc[j] += __shfl_xor_sync(~0u, acc[j], o);
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int j = 0; j < kLowRanks; ++j) part[threadIdx.x >> 5][j] = acc[j];
+  __syncthreads();
+  if (threadIdx.x < kLowRanks) {
+    const int c = c0 + threadIdx.x;
+    float t = 0.0f;
+    if (i >= 0 && c < g.r) {
+      for (int w = 0; w < kLowThreads / 32; ++w) t += part[w][threadIdx.x];
+      t *= g.scale ? g.alpha * g.scale[i] : g.alpha;
+    }
+    if (g.low && c < g.r) g.low[row * g.r + c] = t;
+    if (g.split && c < half) store_split(g.split, row, half, c, t, g.bf16);
+  }
+}
+
+__global__ void k_pad_rows(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd,
+                           int64_t rows, int64_t cols) {
+  const int64_t n = rows * ldd;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / ldd, c = i - r * ldd;
+    dst[i] = c < cols ? src[r * lds + c] : (uint16_t)0;
+  }
+}
+
+}  // namespace
+
+int launch_pad_rows(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows,
+                    int64_t cols, cudaStream_t stream) {
+  if (rows == 0 || cols == 0) return OZK_OK;
+  int64_t blocks = (rows * ldd + 255) / 256;
+  if (blocks > 148 * 16) blocks = 148 * 16;
+  k_pad_rows<<<(unsigned)blocks, 256, 0, stream>>>((const uint16_t*)src, lds, (uint16_t*)dst, ldd,
+                                                   rows, cols);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? OZK_OK : set_cuda_error("k_pad_rows launch", e);
+}
+
+// ---------------------------------------------------------------- launches
+
+namespace {
+
+template <typename... Params, typename... Args>
+int launch_cluster(const char* what, void (*kern)(Params...), int64_t tiles, int splits,
+                   int threads, size_t smem, bool early, cudaStream_t stream, Args... args) {
+  static_assert(sizeof...(Params) == sizeof...(Args), "");
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)smem);
+  if (e != cudaSuccess) return set_cuda_error(what, e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * splits));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? OZK_OK : set_cuda_error(what, e);
+}
+
+struct Operand {
+  const void* p;
+  int64_t ld;
+};
+
+// One product X W^T + (s X A_i^T) B_i^T, or with `back` set the same read the
+// other way: X is dY [M][N], W and the A of the low-rank step lie as [N][K] and
+// [E][N][r] with the contraction along their rows.
+struct Product {
+  Operand X, W, A, B;        // A: the adapters of the first step, B: of the second
+  int64_t M, n_out, n_in;    // rows, output columns, contraction
+  int r, E;
+  bool back, bf16;
+};
+
+int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float alpha, float* low,
+                 uint16_t* split, int32_t* status, int dev, cudaStream_t stream) {
+  LowArgs g = {};
+  g.ids = ids;
+  g.scale = scale;
+  g.alpha = alpha;
+  g.low = low;
+  g.split = split;
+  g.M = p.M;
+  g.E = p.E;
+  g.r = p.r;
+  g.rp = (p.r + 15) / 16 * 16;
+  g.bf16 = p.bf16;
+  g.nkb = (int)((p.n_in + kKB - 1) / kKB);
+  g.status = status;
+  g.budget_ns = wait_budget_ns();
+  if (!p.back && p.M <= 64) {
+    const int half = split_half(p.r);
+    k_low_rank_rows<<<dim3((unsigned)p.M, (unsigned)(half / kLowRanks)), kLowThreads, 0, stream>>>(
+        (const uint16_t*)p.X.p, p.X.ld, (const uint16_t*)p.A.p, p.A.ld, p.n_in, g);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? OZK_OK : set_cuda_error("k_low_rank_rows launch", e);
+  }
+  g.xrows = p.M >= kRows ? kRows : (int)round_up(p.M, 8);
+  const int64_t tiles = (p.M + kRows - 1) / kRows;
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 2 * device_sm_count(dev) && g.nkb >= splits * 4)
+    splits *= 2;
+  const int a_bytes = p.back ? (g.rp + 63) / 64 * 8192 : g.rp * 128;
+  g.xstages = 4;
+  g.astages = 4;
+  size_t area = (size_t)g.xstages * g.xrows * 128 + (size_t)g.astages * a_bytes;
+  // The MMA reads 128 rows of X's last stage even if fewer were loaded.
+  const size_t need = (size_t)(g.xstages - 1) * g.xrows * 128 + kRows * 128;
+  const size_t red = (size_t)kRows * (g.rp + 1) * 4;
+  if (area < need) area = need;
+  if (area < red) area = red;
+  if (area < tmem_share(g.rp)) area = tmem_share(g.rp);
+  CUtensorMap mx, ma;
+  int rc;
+  if ((rc = make_map(&mx, p.X.p, 2, p.n_in, p.M, 1, p.X.ld * 2, p.X.ld * 2 * p.M, kKB, g.xrows,
+                     true)))
+    return rc;
+  if (p.back)
+    rc = make_map(&ma, p.A.p, 2, p.r, p.n_in, p.E, p.A.ld * 2, p.A.ld * 2 * p.n_in, 64, kKB, true);
+  else
+    rc = make_map(&ma, p.A.p, 2, p.n_in, p.r, p.E, p.A.ld * 2, p.A.ld * 2 * p.r, kKB, g.rp, true);
+  if (rc) return rc;
+  return p.back ? launch_cluster("k_low_rank", k_low_rank<true>, tiles, splits, kThreads,
+                                 area + 1024, false, stream, mx, ma, g)
+                : launch_cluster("k_low_rank", k_low_rank<false>, tiles, splits, kThreads,
+                                 area + 1024, false, stream, mx, ma, g);
+}
+
+template <int BN, bool MNB>
+int run_linear_bn(const Product& p, LinearArgs g, const uint16_t* split, int splits,
+                  int dev, cudaStream_t stream) {
+  const int half = split_half(p.r);
+  g.tiles_n = (int)((p.n_out + BN - 1) / BN);
+  const int64_t tiles = (p.M + kRows - 1) / kRows * g.tiles_n;
+  const size_t stage = (size_t)g.xrows * 128 + BN * 128;
+  g.stages = (int)(96 * 1024 / stage);
+  if (g.stages > kMaxStages) g.stages = kMaxStages;
+  size_t area = g.stages * stage;
+  const size_t need = (size_t)(g.stages - 1) * g.xrows * 128 + kRows * 128;
+  const size_t red = (size_t)g.xrows * (BN + 1) * 4;
+  if (area < need) area = need;
+  if (splits > 1 && area < red) area = red;
+  if (area < tmem_share(BN)) area = tmem_share(BN);
+  CUtensorMap mx, mw, mt, mb;
+  int rc;
+  if ((rc = make_map(&mx, p.X.p, 2, p.n_in, p.M, 1, p.X.ld * 2, p.X.ld * 2 * p.M, kKB, g.xrows,
+                     true)))
+    return rc;
+  if ((rc = make_map(&mt, split, 2, 2 * half, p.M, 1, 4 * half, 4 * half * p.M, 64, g.xrows, true)))
+    return rc;
+  if (MNB) {
+    rc = make_map(&mw, p.W.p, 2, p.n_out, p.n_in, 1, p.W.ld * 2, p.W.ld * 2 * p.n_in, 64, kKB, true);
+    if (!rc)
+      rc = make_map(&mb, p.B.p, 2, p.n_out, p.r, p.E, p.B.ld * 2, p.B.ld * 2 * p.r, 64, 64, true);
+  } else {
+    rc = make_map(&mw, p.W.p, 2, p.n_in, p.n_out, 1, p.W.ld * 2, p.W.ld * 2 * p.n_out, kKB, BN,
+                  true);
+    if (!rc)
+      rc = make_map(&mb, p.B.p, 2, p.r, p.n_out, p.E, p.B.ld * 2, p.B.ld * 2 * p.n_out, 64, BN,
+                    true);
+  }
+  if (rc) return rc;
+  return launch_cluster("k_linear", k_linear<BN, MNB>, tiles, splits, kThreads, area + 1024, true,
+                        stream, mx, mw, mt, mb, g);
+}
+
+int run_linear(const Product& p, const int32_t* ids, const uint16_t* split, void* Y, int64_t ldy,
+               int32_t* status, int dev, cudaStream_t stream) {
+  LinearArgs g = {};
+  g.ids = ids;
+  g.Y = Y;
+  g.ldy = ldy;
+  g.M = p.M;
+  g.N = (int)p.n_out;
+  g.nkb = (int)((p.n_in + kKB - 1) / kKB);
+  g.E = p.E;
+  g.r = p.r;
+  g.bf16 = p.bf16;
+  g.y_vec = ((uintptr_t)Y & 15) == 0 && ldy % 8 == 0;
+  g.xrows = p.M >= kRows ? kRows : (int)round_up(p.M, 8);
+  g.status = status;
+  g.budget_ns = wait_budget_ns();
+  const int64_t tiles_m = (p.M + kRows - 1) / kRows;
+  const int sms = device_sm_count(dev);
+  const bool few = tiles_m * ((p.n_out + 127) / 128) < sms;
+  const int64_t tiles = tiles_m * ((p.n_out + (few ? 63 : 127)) / (few ? 64 : 128));
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 2 * sms && g.nkb >= splits * 4) splits *= 2;
+  if (p.back)
+    return few ? run_linear_bn<64, true>(p, g, split, splits, dev, stream)
+               : run_linear_bn<128, true>(p, g, split, splits, dev, stream);
+  return few ? run_linear_bn<64, false>(p, g, split, splits, dev, stream)
+             : run_linear_bn<128, false>(p, g, split, splits, dev, stream);
+}
+
+// Copies an operand that TMA cannot read into the workspace, its rows padded
+// to 16 bytes; `launch` false only counts the bytes.
+int align_operand(Operand& o, int64_t rows, int64_t cols, Arena& ws, bool launch,
+                  cudaStream_t stream) {
+  if (tma_ready(o.p, o.ld)) return OZK_OK;
+  const int64_t ld = round_up(cols, 8);
+  void* d = ws.take<void>((size_t)(rows * ld * 2));
+  if (launch) {
+    int rc = launch_pad_rows(o.p, o.ld, d, ld, rows, cols, stream);
+    if (rc) return rc;
+  }
+  o.p = d;
+  o.ld = ld;
+  return OZK_OK;
+}
+
+}  // namespace
+
+}  // namespace ozk
+
+using namespace ozk;
+
+static int adapter_args(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* A,
+                        const void* B, int64_t M, int64_t N, int64_t K, int r, int E, int dt) {
+  if (!dt_is_16bit(dt)) return set_error(OZK_ERR_ARG, "dtype must be OZK_DT_BF16 or OZK_DT_F16");
+  if (M < 0 || N < 0 || K < 1) return set_error(OZK_ERR_ARG, "need M, N >= 0 and K >= 1");
+  if (M > (1 << 30) || N > (1 << 30) || K > (1 << 30))
+    return set_error(OZK_ERR_UNSUPPORTED, "M, N and K are limited to 2^30");
+  if (r < 1 || r > kMaxRank)
+    return set_error(OZK_ERR_ARG, "rank %d; expected 1 to %d", r, kMaxRank);
+  if (E < 1 || E > (1 << 20)) return set_error(OZK_ERR_ARG, "need 1 <= E <= 2^20 adapters");
+  if (M == 0 || N == 0) return OZK_OK;
+  if (!X || !W || !A || !B) return set_error(OZK_ERR_ARG, "NULL pointer");
+  if (ldw < K) return set_error(OZK_ERR_ARG, "ldw < K");
+  return OZK_OK;
+}
+
+extern "C" {
+
+size_t ozk_matmul_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E) {
+  if (M < 1 || N < 1 || K < 1 || r < 1 || r > kMaxRank || E < 1) return 0;
+  Arena ws(nullptr);
+  ws.take<uint16_t>((size_t)M * 4 * split_half(r));
+  // The worst case: every operand has to be copied to be aligned.
+  ws.take((size_t)M * round_up(K, 8) * 2);
+  ws.take((size_t)N * round_up(K, 8) * 2);
+  ws.take((size_t)E * r * round_up(K, 8) * 2);
+  ws.take((size_t)E * N * round_up(r, 8) * 2);
+  return ws.used;
+}
+
+int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* A,
+                        const void* B, const int32_t* ids, const float* scale, double alpha,
+                        void* Y, int64_t ldy, float* low, int64_t M, int64_t N, int64_t K, int r,
+                        int E, int dt, void* workspace, size_t ws_bytes, int32_t* status_dev,
+                        void* stream) {
+  int rc = adapter_args(X, ldx, W, ldw, A, B, M, N, K, r, E, dt);
+  if (rc) return rc;
+  if (M == 0 || N == 0) return OZK_OK;
+  if (ldx < K) return set_error(OZK_ERR_ARG, "ldx < K");
+  if (!Y || ldy < N) return set_error(OZK_ERR_ARG, "NULL Y or ldy < N");
+  cudaStream_t s = (cudaStream_t)stream;
+  int dev;
+  cudaGetDevice(&dev);
+  Product p = {{X, ldx}, {W, ldw}, {A, K}, {B, r}, M, N, K, r, E, false, dt == OZK_DT_BF16};
+  Arena ws(workspace);
+  uint16_t* split = ws.take<uint16_t>((size_t)M * 4 * split_half(r));
+  for (int pass = 0; pass < 2; ++pass) {  // count first, then copy
+    Product q = p;
+    Arena w = ws;
+    if ((rc = align_operand(q.X, M, K, w, pass, s)) || (rc = align_operand(q.W, N, K, w, pass, s)) ||
+        (rc = align_operand(q.A, (int64_t)E * r, K, w, pass, s)) ||
+        (rc = align_operand(q.B, (int64_t)E * N, r, w, pass, s)))
+      return rc;
+    if (pass) p = q;
+    else if (!workspace || w.used > ws_bytes || ((uintptr_t)workspace & 127))
+      return set_error(OZK_ERR_WORKSPACE, "workspace of %zu bytes, aligned to 128, needed", w.used);
+  }
+  if ((rc = run_low_rank(p, ids, scale, (float)alpha, low, split, status_dev, dev, s))) return rc;
+  return run_linear(p, ids, split, Y, ldy, status_dev, dev, s);
+}
+
+}  // extern "C"

@@ -35,6 +35,7 @@
 #include "ozk_device.cuh"
 #include "ozk_fixed.cuh"
 #include "ozk_internal.h"
+#include "ozk_tile16.cuh"
 
 namespace ozk {
 
@@ -887,6 +888,23 @@ int make_slice_map(CUtensorMap* map, const void* base, int64_t k_pad, int64_t ro
   CUresult r = g_encode(map, s8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                         3, (void*)base, dims, strides, box,
                         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(OZK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return OZK_OK;
+}
+
+// Tensor map of a [d2][d1][d0] array (see ozk_tile16.cuh).
+int make_map(CUtensorMap* map, const void* base, int esz, int64_t d0, int64_t d1, int64_t d2,
+             int64_t s1, int64_t s2, int b0, int b1, bool swz) {
+  int rc = get_encode_fn();
+  if (rc) return rc;
+  cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
+  cuuint64_t strides[2] = {(cuuint64_t)s1, (cuuint64_t)s2};
+  cuuint32_t box[3] = {(cuuint32_t)b0, (cuuint32_t)b1, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, esz == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                        3, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swz ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(OZK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return OZK_OK;
