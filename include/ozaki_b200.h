@@ -447,6 +447,31 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
                         int E, int dt, void* workspace, size_t ws_bytes, int32_t* status_dev,
                         void* stream);
 
+/* Rows of X [M][K] (ldx, type dt: any OZK_DT_*) as int8 codes and exponents.
+ * A group of 128 columns of a row shares the step 2^e, the smallest power of
+ * two under which its largest magnitude rounds to at most 127;
+ * code = RN(x / 2^e).  e is held to [-126, 121] (OZK_DT_F16: [-24, 9]); at the
+ * upper end codes saturate at +-127.  A group holding a NaN or an infinity has
+ * e = -128 and restores as NaN.  codes: int8 [M][ldc], ldc = K rounded up to
+ * 128, 16-byte aligned, 0 beyond column K; exps: int8 [ceil(K / 128)][M].
+ * At most 2097120 rows. */
+int ozk_checkpoint_rows(const void* X, int64_t ldx, int64_t M, int64_t K, int dt, void* codes,
+                        int64_t ldc, void* exps, void* stream);
+/* The values code * 2^e of a checkpoint in type dt (exact in the type the
+ * checkpoint was made from, and in OZK_DT_F32). */
+int ozk_restore_rows(const void* codes, int64_t ldc, const void* exps, int64_t M, int64_t K,
+                     void* out, int64_t ldo, int dt, void* stream);
+/* Weight gradient from a checkpointed input: out = dY^T X^ (+ out with
+ * accumulate), dY [M][N] (ldy, type dt: OZK_DT_BF16 or OZK_DT_F16), X^ [M][K]
+ * the restored rows, out [N][K] (ldo) of type out_dt (dt or OZK_DT_F32).  FP32
+ * sums, one rounding.  The result does not depend on scheduling: where the
+ * rows are split, the parts are added in order. */
+size_t ozk_checkpoint_grad_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int ozk_checkpoint_grad(const void* dY, int64_t ldy, const void* codes, int64_t ldc,
+                        const void* exps, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                        int dt, int out_dt, int accumulate, void* workspace, size_t ws_bytes,
+                        int32_t* status_dev, void* stream);
+
 /* Library version string. */
 const char* ozk_version(void);
 

@@ -19,6 +19,7 @@ from .extract import (
     jax_extract_split_rows, jax_extract_split_cols,
 )
 from .adapters import matmul_adapters
+from .checkpoint import SavedRows, checkpoint_rows, restore_rows, checkpoint_grad
 from .accum import accumulate_2sum, validate_accumulation_2sum
 
 __all__ = [
@@ -26,6 +27,7 @@ __all__ = [
     "extract_split_rows", "extract_split_cols",
     "f32_extract_split_rows", "f32_extract_split_cols",
     "jax_extract_split_rows", "jax_extract_split_cols",
+    "SavedRows", "checkpoint_rows", "restore_rows", "checkpoint_grad",
     "matmul_adapters",
     "accumulate_2sum", "validate_accumulation_2sum",
     "compute_rho_f32", "compute_rho_f64", "ondevice_safety_report",

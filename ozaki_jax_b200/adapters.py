@@ -50,10 +50,12 @@ def check_device(device, **tensors):
 
 
 def row_major(x):
-    """x with its columns adjacent and its rows not overlapping (copied only when needed)."""
-    if x.stride(1) == 1 and x.stride(0) >= x.shape[1]:
-        return x
-    return x.contiguous()
+    """(x, its row stride) with adjacent columns and rows that do not overlap
+    (copied only when needed; a stride along one element counts for nothing)."""
+    rows, cols = x.shape
+    if (x.stride(1) == 1 or cols <= 1) and (x.stride(0) >= cols or rows <= 1):
+        return x, x.stride(0) if rows > 1 else max(cols, 1)
+    return x.contiguous(), max(cols, 1)
 
 
 def _adapter_shapes(W, A, B, ids, scale, rows, dtype):
@@ -117,7 +119,8 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
     dev = X.device
     factors, alpha = _scale_args(scale)
     check_device(dev, W=W, A=A, B=B, ids=ids, scale=factors)
-    X, W, A, B = row_major(X), row_major(W), A.contiguous(), B.contiguous()
+    (X, ldx), (W, ldw) = row_major(X), row_major(W)
+    A, B = A.contiguous(), B.contiguous()
     ids = None if ids is None else ids.contiguous()
     Y = torch.empty((M, N), dtype=X.dtype, device=dev)
     low = torch.empty((M, r), dtype=torch.float32, device=dev) if return_low else None
@@ -127,7 +130,7 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         with D.on_device(dev):
             L.check(lib.ozk_matmul_adapters(
-                X.data_ptr(), X.stride(0), W.data_ptr(), W.stride(0), A.data_ptr(), B.data_ptr(),
+                X.data_ptr(), ldx, W.data_ptr(), ldw, A.data_ptr(), B.data_ptr(),
                 _ptr(ids), _ptr(factors), alpha, Y.data_ptr(), N, _ptr(low), M, N, K, r, E,
                 DTYPES[X.dtype], ws.data_ptr(), n, None, D.stream_handle(dev)))
     elif low is not None:

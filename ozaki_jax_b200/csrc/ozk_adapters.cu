@@ -38,10 +38,6 @@ constexpr int kMaxRank = 128;
 constexpr int kMaxStages = 16;
 constexpr int kThreads = 192;    // producer warp, MMA warp, four epilogue warps
 
-// Columns of the split T of rank r: [hi 32 | lo 32] up to rank 32, else the
-// high parts of ceil(r / 64) blocks of 64, then the low parts.
-__host__ __device__ inline int split_half(int r) { return r <= 32 ? 32 : (r + 63) / 64 * 64; }
-
 struct LinearArgs {
   const int32_t* ids;
   void* Y;
@@ -52,20 +48,6 @@ struct LinearArgs {
   int stages, xrows, tiles_n;
   int32_t* status;
   uint64_t budget_ns;
-};
-
-// Ring of shared-memory stages: the index and phase parity of step `it`.
-struct Ring {
-  int n;
-  int s = 0;
-  uint32_t ph = 0;
-  __device__ explicit Ring(int stages) : n(stages) {}
-  __device__ void next() {
-    if (++s == n) {
-      s = 0;
-      ph ^= 1;
-    }
-  }
 };
 
 // 8 or 16 consecutive output columns of one row.

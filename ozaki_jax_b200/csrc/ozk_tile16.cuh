@@ -85,6 +85,79 @@ __device__ __forceinline__ float widen16(bool bf16, uint16_t u) {
   return bf16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
 }
 
+// mbar_wait that also acquires what a peer CTA's threads wrote before their
+// (cluster-scope) arrivals.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
+                                                  volatile int* abort, int32_t* status,
+                                                  uint64_t budget_ns) {
+  if (!mbar_wait(bar, parity, abort, status, budget_ns)) return false;
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return true;
+}
+
+// Ring of shared-memory stages: the index and phase parity of the current step.
+struct Ring {
+  int n;
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ explicit Ring(int stages) : n(stages) {}
+  __device__ void next() {
+    if (++s == n) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+};
+
+// Columns of the split T of rank r, high or low half: 32 up to rank 32, else
+// ceil(r / 64) blocks of 64.
+__host__ __device__ inline int split_half(int r) { return r <= 32 ? 32 : (r + 63) / 64 * 64; }
+
+// ------------------------------------------------- int8 checkpoint codes
+
+constexpr int kGroup = 128;      // columns of a row that share an exponent
+constexpr int kExpNaN = -128;    // exponent of a group that held a NaN or infinity
+
+// 2^e as a packed pair of 16-bit values (NaN for kExpNaN): exact for the
+// exponents that checkpoint_rows writes for the type.
+__device__ __forceinline__ uint32_t exp_pair(bool bf16, int e) {
+  if (e == kExpNaN) return bf16 ? 0x7FC07FC0u : 0x7E007E00u;
+  const float f = pow2f(e);
+  return pack16(bf16, f, f);
+}
+
+// Four int8 codes times 2^e as two packed pairs, exactly.
+// BF16 holds 128 + m exactly for m in [0, 127] (0x4300 | m), so with the code
+// q = (q & 127) - 128 [q < 0]: q = (0x4300 | (q & 127)) - (0x4300 | (q & 128)),
+// the second being 128 or 256.  FP16 holds 1024 + u for a byte u (0x6400 | u):
+// q = (0x6400 | (q ^ 128)) - 1152.
+__device__ __forceinline__ void codes_to_16(bool bf16, uint32_t q4, uint32_t scale, uint32_t& lo,
+                                            uint32_t& hi) {
+  if (bf16) {
+    const uint32_t a = __byte_perm(q4, 0x43434343u, 0x4140);
+    const uint32_t b = __byte_perm(q4, 0x43434343u, 0x4342);
+    const uint32_t a0 = a & 0xFF7FFF7Fu, a1 = a & 0xFF80FF80u;
+    const uint32_t b0 = b & 0xFF7FFF7Fu, b1 = b & 0xFF80FF80u;
+    const __nv_bfloat162 s = *(const __nv_bfloat162*)&scale;
+    const __nv_bfloat162 x =
+        __hmul2(__hsub2(*(const __nv_bfloat162*)&a0, *(const __nv_bfloat162*)&a1), s);
+    const __nv_bfloat162 y =
+        __hmul2(__hsub2(*(const __nv_bfloat162*)&b0, *(const __nv_bfloat162*)&b1), s);
+    lo = *(const uint32_t*)&x;
+    hi = *(const uint32_t*)&y;
+  } else {
+    const uint32_t u = q4 ^ 0x80808080u;
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140);
+    const uint32_t b = __byte_perm(u, 0x64646464u, 0x4342);
+    const uint32_t c = 0x64806480u;  // 1152
+    const __half2 s = *(const __half2*)&scale;
+    const __half2 x = __hmul2(__hsub2(*(const __half2*)&a, *(const __half2*)&c), s);
+    const __half2 y = __hmul2(__hsub2(*(const __half2*)&b, *(const __half2*)&c), s);
+    lo = *(const uint32_t*)&x;
+    hi = *(const uint32_t*)&y;
+  }
+}
+
 // ------------------------------------------------- adapters of a row tile
 
 // Adapter of row `row`: -1 for none (an id outside [0, E)).  Without ids every
@@ -144,6 +217,38 @@ int make_map(CUtensorMap* map, const void* base, int esz, int64_t d0, int64_t d1
 inline bool tma_ready(const void* p, int64_t ld) {
   return ((uintptr_t)p & 15) == 0 && (ld * 2) % 16 == 0;
 }
+
+// 256 x 256 tiles on CTA pairs (ozk_wide16.cu).
+enum WideMode {
+  kWideForward = 0,  // A [M][C], B [N][C]: both operands' rows run along the contraction C
+  kWideBack = 1,     // A [M][C], B [C][N]
+  kWideWeight = 2    // A [C][M], B [C][N] as int8 codes and exponents
+};
+struct WideProduct {
+  WideMode mode;
+  bool bf16;
+  int64_t M, N, C;
+  const void* A;
+  int64_t lda;
+  const void* B;           // 16-bit elements, or int8 codes
+  int64_t ldb;
+  const int8_t* exps;      // kWideWeight: [ceil(N / 128)][C]
+  // Further contraction: adapters' T B_i^T (kWideForward, kWideBack), r = 0: none.
+  const int32_t* ids;
+  int r, E;
+  const uint16_t* split;   // [M][2 split_half(r)]
+  const void* Bi;          // [E][N][r] (forward) or [E][r][N] (back)
+  int64_t ldbi;
+  bool early;              // launch while the kernel before it (which writes split) still runs
+  void* out;               // [M][N], 16-bit of the operands' type or FP32
+  int64_t ldo;
+  bool out_f32, accumulate;
+  float* partial;          // kWideWeight: room for wide_partial_bytes, or NULL
+  int32_t* status;
+};
+int launch_wide(const WideProduct& p, int dev, cudaStream_t stream);
+// Scratch of a kWideWeight product: FP32 partials when its contraction is split.
+size_t wide_partial_bytes(int64_t M, int64_t N, int64_t C, int dev);
 
 // Shared memory that a CTA of these kernels asks for at least when it holds
 // `cols` TMEM columns: its share of the SM's 227 KB.  CTAs that fit an SM

@@ -1,0 +1,581 @@
+// k_wide: 16-bit products on 256 x 256 tiles of CTA pairs, FP32 accumulators.
+//
+//   forward  Y  = X W^T  (+ T B_i^T)     both operands K-major
+//   back     dX = dY W   (+ U A_i)       W and A_i MN-major
+//   weight   dW = dY^T X^                dY MN-major, X^ from int8 codes
+//
+// Bound by the tensor cores.  Persistent: each CTA pair (cta_group::2, M = 256)
+// walks its tiles; each CTA stages its 128 rows of A and half of B's 256
+// columns per 64 contraction indexes (32 KB), so a stage is read from shared
+// memory at 64 B/clk, half of what the two CTAs would read apart.  Two TMEM
+// accumulators (all 512 columns) let the epilogue of one tile run under the
+// MMAs of the next.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (one thread of the even CTA), 2-5
+// epilogue, 6 the tile's list of adapters (forward, back) or 6-13 (weight)
+// the converters, which turn each CTA's 128 columns x 64 rows of codes (TMA'd
+// into a ring of their own) into 16-bit values in the MMA's layout: 16 codes
+// per clock and SM at the MMA's full rate, at about 2.5 instructions a code.
+// The exponents are powers of two, so a code times its step is exact in the
+// operand type and the product is that of the restored matrix.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "ozk_tile16.cuh"
+
+namespace ozk {
+
+namespace {
+
+constexpr int kTile = 256;
+constexpr int kHalf = 128;       // rows of A, columns of B per CTA
+constexpr int kKB = 64;          // contraction indexes per stage
+constexpr int kABytes = kHalf * kKB * 2;
+constexpr int kStageBytes = 2 * kABytes;
+constexpr int kRawBytes = kHalf * kKB;
+constexpr int kConvWarps = 8;
+
+template <WideMode MODE>
+struct WideCfg {
+  static constexpr bool W = MODE == kWideWeight;
+  static constexpr int STAGES = W ? 5 : 6;
+  static constexpr int RAW = W ? 6 : 0;
+  static constexpr int THREADS = W ? 32 * (6 + kConvWarps) : 32 * 7;
+  // All of an SM's shared memory: a CTA holds all TMEM columns, so no other
+  // TMEM kernel may share the SM.
+  static constexpr int SMEM = 227 * 1024 - (W ? 1024 : 11 * 1024);
+};
+
+struct WideArgs {
+  int64_t M, N;
+  int nkb, tiles_m, tiles_n, group_m, splits;
+  int bf16, out_f32, accumulate, o_vec;
+  void* out;
+  int64_t ldo;
+  float* partial;      // [splits][M][N] when splits > 1
+  const int8_t* exps;  // [groups][C]
+  int64_t C;
+  const int32_t* ids;
+  int r, E;
+  int32_t* status;
+  uint64_t budget_ns;
+};
+
+// Tiles walk down groups of group_m tile rows before moving right, so the
+// tiles in flight share few panels.
+__device__ __forceinline__ void tile_at(const WideArgs& g, int t, int& tm, int& tn) {
+  const int per = g.group_m * g.tiles_n;
+  const int grp = t / per, first = grp * g.group_m;
+  const int rows = g.tiles_m - first < g.group_m ? g.tiles_m - first : g.group_m;
+  const int r = t - grp * per;
+  tm = first + r % rows;
+  tn = r / rows;
+}
+
+// 32 consecutive outputs of one row, n of them inside the matrix.
+__device__ __forceinline__ void store_row(const WideArgs& g, int64_t row, int64_t col, int n,
+                                          const uint32_t (&v)[32]) {
+  if (g.out_f32) {
+    float* o = (float*)g.out + row * g.ldo + col;
+    if (g.o_vec && n >= 32) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        float4 q = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]),
+                               __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+        if (g.accumulate) {
+          const float4 p = *(const float4*)(o + i);
+          q.x += p.x, q.y += p.y, q.z += p.z, q.w += p.w;
+        }
+        *(float4*)(o + i) = q;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < n) o[i] = __uint_as_float(v[i]) + (g.accumulate ? o[i] : 0.0f);
+    }
+  } else {
+    uint16_t* o = (uint16_t*)g.out + row * g.ldo + col;
+    if (g.o_vec && n >= 32) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[i + j]);
+        if (g.accumulate) {
+          const uint4 p = *(const uint4*)(o + i);
+          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f[2 * j] += widen16(g.bf16, (uint16_t)w[j]);
+            f[2 * j + 1] += widen16(g.bf16, (uint16_t)(w[j] >> 16));
+          }
+        }
+        uint4 q;
+        q.x = pack16(g.bf16, f[0], f[1]);
+        q.y = pack16(g.bf16, f[2], f[3]);
+        q.z = pack16(g.bf16, f[4], f[5]);
+        q.w = pack16(g.bf16, f[6], f[7]);
+        *(uint4*)(o + i) = q;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < n)
+          o[i] = round16(g.bf16, __uint_as_float(v[i]) + (g.accumulate ? widen16(g.bf16, o[i]) : 0.0f));
+    }
+  }
+}
+
+template <WideMode MODE>
+__global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
+    k_wide(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
+           const __grid_constant__ CUtensorMap mapT, const __grid_constant__ CUtensorMap mapBi,
+           const __grid_constant__ WideArgs g) {
+  using Cfg = WideCfg<MODE>;
+  constexpr int STAGES = Cfg::STAGES, RAW = Cfg::RAW;
+  constexpr bool AMN = MODE == kWideWeight, BMN = MODE != kWideForward;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sRaw = smem + STAGES * kStageBytes;
+  __shared__ uint64_t full[STAGES], empty[STAGES], rfull[RAW + 1], rempty[RAW + 1], accf[2],
+      acce[2], sfull, sempty, done;
+  __shared__ SlotList<MODE == kWideWeight ? 1 : 8> slots;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort_word;
+  volatile int* s_abort = &s_abort_word;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int unit = (int)(blockIdx.x >> 1), n_units = (int)(gridDim.x >> 1);
+  const int tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits;
+  const int half = split_half(g.r);
+  const int blocks = half < 64 ? 1 : half / 64 * 2;  // stages per adapter
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], MODE == kWideWeight ? 1 + 2 * kConvWarps : 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < RAW; ++i) {
+      mbar_init(&rfull[i], 1);
+      mbar_init(&rempty[i], kConvWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&accf[i], 1);
+      mbar_init(&acce[i], 2 * 4);
+    }
+    mbar_init(&sfull, 1);
+    mbar_init(&sempty, rank == 0 ? 2 : 1);
+    mbar_init(&done, 1);
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_pair(&s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  auto item_at = [&](int i, int& tm, int& tn, int& sp, int& kb0, int& kb1) {
+    sp = i / tiles;
+    tile_at(g, i - sp * tiles, tm, tn);
+    kb0 = (int)((int64_t)g.nkb * sp / g.splits);
+    kb1 = (int)((int64_t)g.nkb * (sp + 1) / g.splits);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      Ring rg(STAGES), rr(RAW > 0 ? RAW : 1);
+      bool ok = true, waited = false;
+      int issued = 0, raws = 0;
+      uint32_t sph = 0;
+      for (int i = unit; ok && i < items; i += n_units) {
+        int tm, tn, sp, kb0, kb1;
+        item_at(i, tm, tn, sp, kb0, kb1);
+        const int arow = tm * kTile + (int)rank * kHalf;
+        const int bcol = tn * kTile + (int)rank * kHalf;
+        auto load = [&](const CUtensorMap* ma, int ax, const CUtensorMap* mb, int bx, int bz) {
+          if (!mbar_wait(&empty[rg.s], rg.ph ^ 1, s_abort, g.status, g.budget_ns)) return false;
+          if (rank == 0)
+            mbar_arrive_expect_tx(&full[rg.s], 2 * (MODE == kWideWeight ? kABytes : kStageBytes));
+          const uint32_t fb = mapa_u32(&full[rg.s], 0);
+          uint8_t* a = smem + rg.s * kStageBytes;
+          uint8_t* b = a + kABytes;
+          if constexpr (AMN) {
+            tma_load_3d_pair(a, ma, fb, arow, ax, 0);
+            tma_load_3d_pair(a + 8192, ma, fb, arow + 64, ax, 0);
+          } else {
+            tma_load_3d_pair(a, ma, fb, ax, arow, 0);
+          }
+          if constexpr (MODE == kWideForward) {
+            tma_load_3d_pair(b, mb, fb, bx, bcol, bz);
+          } else if constexpr (MODE == kWideBack) {
+            tma_load_3d_pair(b, mb, fb, bcol, bx, bz);
+            tma_load_3d_pair(b + 8192, mb, fb, bcol + 64, bx, bz);
+          }
+          rg.next();
+          ++issued;
+          return true;
+        };
+        for (int kb = kb0; ok && kb < kb1; ++kb) {
+          if constexpr (MODE == kWideWeight) {
+            if (!mbar_wait(&rempty[rr.s], rr.ph ^ 1, s_abort, g.status, g.budget_ns)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&rfull[rr.s], kRawBytes);
+            tma_load_3d(sRaw + rr.s * kRawBytes, &mapB, &rfull[rr.s], bcol, kb * kKB, 0);
+            rr.next();
+            ++raws;
+          }
+          ok = load(&mapA, kb * kKB, &mapB, kb * kKB, 0);
+        }
+        if (MODE != kWideWeight && g.r > 0) {
+          if (!waited) grid_wait();  // the split T comes from the kernel before this one
+          waited = true;
+          ok = ok && mbar_wait(&sfull, sph, s_abort, g.status, g.budget_ns);
+          const int n = ok ? slots.n : 0;
+          for (int j = 0; ok && j < n; ++j)
+            for (int b = 0; ok && b < blocks; ++b)
+              ok = load(&mapT, blocks == 1 ? 0 : (b & 1) * half + (b >> 1) * 64, &mapBi,
+                        blocks == 1 ? 0 : (b >> 1) * 64, slots.id[j]);
+          if (ok) mbar_arrive(&sempty);
+          sph ^= 1;
+        }
+      }
+      if (!waited) grid_wait();
+      // Drain: every copy lands before shared memory is released (the even
+      // CTA's full barriers count both CTAs' bytes).
+      if (rank == 0) {
+        Ring b(STAGES);
+        for (int i = 0; i < issued; ++i, b.next())
+          if (i >= issued - STAGES) mbar_wait(&full[b.s], b.ph, nullptr, g.status, g.budget_ns);
+      }
+      Ring b(RAW > 0 ? RAW : 1);
+      for (int i = 0; i < raws; ++i, b.next())
+        if (i >= raws - RAW) mbar_wait(&rfull[b.s], b.ph, nullptr, g.status, g.budget_ns);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = umma_idesc_16(g.bf16, kTile, kTile, AMN, BMN);
+      Ring rg(STAGES);
+      bool ok = true;
+      int it = 0;
+      uint32_t sph = 0;
+      auto desc_a = [](uint32_t a, int kk) {
+        return AMN ? umma_desc_mn128(a + kk * 2048, 8192) : umma_desc_sw128(a + kk * 32);
+      };
+      auto desc_b = [](uint32_t b, int kk) {
+        return BMN ? umma_desc_mn128(b + kk * 2048, 8192) : umma_desc_sw128(b + kk * 32);
+      };
+      for (int i = unit; ok && i < items; i += n_units, ++it) {
+        int tm, tn, sp, kb0, kb1;
+        item_at(i, tm, tn, sp, kb0, kb1);
+        const int buf = it & 1;
+        ok = mbar_wait(&acce[buf], ((it >> 1) & 1) ^ 1, s_abort, g.status, g.budget_ns);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * kTile;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = MODE == kWideWeight
+                   ? mbar_wait_cluster(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns)
+                   : mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(smem + rg.s * kStageBytes), b0 = a0 + kABytes;
+#pragma unroll
+          for (int kk = 0; kk < kKB / 16; ++kk)
+            umma_bf16_pair(d, desc_a(a0, kk), desc_b(b0, kk), idesc, kb != kb0 || kk != 0);
+          umma_commit_pair(&empty[rg.s], 0x3);
+          rg.next();
+        }
+        if constexpr (MODE != kWideWeight) {
+          if (g.r > 0) {
+            ok = ok && mbar_wait(&sfull, sph, s_abort, g.status, g.budget_ns);
+            const int n = ok ? slots.n : 0;
+            for (int j = 0; ok && j < n; ++j) {
+              uint32_t off[8];
+#pragma unroll
+              for (int w = 0; w < 8; ++w) off[w] = slots.off[j][w];
+              for (int b = 0; b < blocks; ++b) {
+                ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t a0 = smem_u32(smem + rg.s * kStageBytes), b0 = a0 + kABytes;
+                const int left = g.r - (b >> 1) * 64;
+                const int steps = left >= 64 ? 4 : (left + 15) / 16;
+                for (int kk = 0; kk < steps; ++kk) {
+                  umma_16_masked_pair(d, desc_a(a0, kk), desc_b(b0, kk), idesc, 1, off);
+                  if (blocks == 1)
+                    umma_16_masked_pair(d, umma_desc_sw128(a0 + 64 + kk * 32), desc_b(b0, kk),
+                                        idesc, 1, off);
+                }
+                umma_commit_pair(&empty[rg.s], 0x3);
+                rg.next();
+              }
+            }
+            if (ok) mbar_arrive(&sempty);
+            sph ^= 1;
+          }
+        }
+        if (!ok) break;
+        umma_commit_pair(&accf[buf], 0x3);
+      }
+      umma_commit_pair(&done, 0x1);
+      mbar_wait(&done, 0, nullptr, g.status, g.budget_ns);
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;
+    int it = 0;
+    for (int i = unit; i < items; i += n_units, ++it) {
+      int tm, tn, sp, kb0, kb1;
+      item_at(i, tm, tn, sp, kb0, kb1);
+      const int buf = it & 1;
+      if (!mbar_wait(&accf[buf], (it >> 1) & 1, s_abort, g.status, g.budget_ns)) break;
+      tc_fence_after();
+      const int64_t row = (int64_t)tm * kTile + rank * kHalf + q * 32 + lane;
+      const int64_t col0 = (int64_t)tn * kTile;
+      const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + buf * kTile;
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(acc + c, v);
+        tmem_wait_ld();
+        if (c == kTile - 32) {
+          // The accumulator is read: the tile after the next may start.
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_u32(&acce[buf], 0));
+        }
+        const int64_t left = g.N - (col0 + c);
+        if (row >= g.M || left <= 0) continue;
+        const int n = left < 32 ? (int)left : 32;
+        if (g.splits > 1) {
+          float* o = g.partial + ((int64_t)sp * g.M + row) * g.N + col0 + c;
+          if (n == 32 && (g.N & 3) == 0) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              *(float4*)(o + j) = make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]),
+                                              __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < n) o[j] = __uint_as_float(v[j]);
+          }
+        } else {
+          store_row(g, row, col0 + c, n, v);
+        }
+      }
+    }
+  } else if constexpr (MODE == kWideWeight) {
+    // ------------------------------------------------------------ converters
+    // Thread: rows t / 16 + 16 j of the stage, 8 columns at 8 (t % 16); lanes of
+    // a half warp write one row's 16-byte pieces, eight to a 128-byte line.
+    const int t = threadIdx.x - 192;
+    const int piece = t & 15, r0 = t >> 4;
+    const uint32_t to = smem_u32(smem) + kABytes + (piece >> 3) * 8192;
+    Ring rg(STAGES), rr(RAW);
+    bool ok = true;
+    for (int i = unit; ok && i < items; i += n_units) {
+      int tm, tn, sp, kb0, kb1;
+      item_at(i, tm, tn, sp, kb0, kb1);
+      const int64_t group = (int64_t)tn * 2 + rank;
+      const bool inside = group * kGroup < g.N;
+      const int8_t* ex = g.exps + (inside ? group * g.C : 0);
+      auto exp_of = [&](int kb, int j) {
+        const int64_t m = (int64_t)kb * kKB + r0 + 16 * j;
+        return inside && m < g.C ? (int)__ldg(ex + m) : -127;
+      };
+      int e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = exp_of(kb0, j);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        int en[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) en[j] = kb + 1 < kb1 ? exp_of(kb + 1, j) : 0;
+        ok = mbar_wait(&rfull[rr.s], rr.ph, s_abort, g.status, g.budget_ns);
+        if (!ok) break;
+        uint2 q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          q[j] = *(const uint2*)(sRaw + rr.s * kRawBytes + (r0 + 16 * j) * kHalf + piece * 8);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&rempty[rr.s]);
+        ok = mbar_wait(&empty[rg.s], rg.ph ^ 1, s_abort, g.status, g.budget_ns);
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = r0 + 16 * j;
+          const uint32_t sc = exp_pair(g.bf16, e[j]);
+          uint32_t w[4];
+          codes_to_16(g.bf16, q[j].x, sc, w[0], w[1]);
+          codes_to_16(g.bf16, q[j].y, sc, w[2], w[3]);
+          const uint32_t at = to + rg.s * kStageBytes + row * 128 +
+                              (((uint32_t)(piece & 7) ^ (uint32_t)(row & 7)) << 4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
+                       "r"(w[2]), "r"(w[3])
+                       : "memory");
+          e[j] = en[j];
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_u32(&full[rg.s], 0));
+        rg.next();
+        rr.next();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ adapter lists
+    uint32_t ph = 0;
+    for (int i = unit; g.r > 0 && i < items; i += n_units) {
+      int tm, tn, sp, kb0, kb1;
+      item_at(i, tm, tn, sp, kb0, kb1);
+      if (!mbar_wait(&sempty, ph ^ 1, s_abort, g.status, g.budget_ns)) break;
+      build_slots<8>(g.ids, (int64_t)tm * kTile, g.M, g.E, (SlotList<8>*)(void*)&slots, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sfull);
+      ph ^= 1;
+    }
+  }
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// Sum of the contraction's parts, in order, into the output.
+__global__ void k_wide_join(const float* part, int splits, int64_t M, int64_t N, void* out,
+                            int64_t ldo, int out_f32, int bf16, int accumulate) {
+  const int64_t n = M * N;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    float s = 0.0f;
+    for (int q = 0; q < splits; ++q) s += part[q * n + i];
+    const int64_t r = i / N, at = r * ldo + (i - r * N);
+    if (out_f32) {
+      float* o = (float*)out + at;
+      *o = s + (accumulate ? *o : 0.0f);
+    } else {
+      uint16_t* o = (uint16_t*)out + at;
+      *o = round16(bf16, s + (accumulate ? widen16(bf16, *o) : 0.0f));
+    }
+  }
+}
+
+// Parts of a weight product's contraction: as many as give every CTA pair a
+// tile, each of at least 8 stages (512 indexes).
+int wide_splits(int64_t M, int64_t N, int64_t C, int dev) {
+  const int64_t tiles = ((M + kTile - 1) / kTile) * ((N + kTile - 1) / kTile);
+  const int units = device_sm_count(dev) / 2;
+  const int64_t nkb = (C + kKB - 1) / kKB;
+  int64_t s = units / tiles;
+  if (s > nkb / 8) s = nkb / 8;
+  return s < 2 ? 1 : (int)s;
+}
+
+template <WideMode MODE>
+int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) {
+  using Cfg = WideCfg<MODE>;
+  CUtensorMap ma, mb, mt, mbi;
+  memset(&mt, 0, sizeof(mt));
+  memset(&mbi, 0, sizeof(mbi));
+  int rc;
+  if (MODE == kWideWeight)
+    rc = make_map(&ma, p.A, 2, p.M, p.C, 1, p.lda * 2, p.lda * 2 * p.C, 64, kKB, true);
+  else
+    rc = make_map(&ma, p.A, 2, p.C, p.M, 1, p.lda * 2, p.lda * 2 * p.M, kKB, kHalf, true);
+  if (rc) return rc;
+  if (MODE == kWideForward)
+    rc = make_map(&mb, p.B, 2, p.C, p.N, 1, p.ldb * 2, p.ldb * 2 * p.N, kKB, kHalf, true);
+  else if (MODE == kWideBack)
+    rc = make_map(&mb, p.B, 2, p.N, p.C, 1, p.ldb * 2, p.ldb * 2 * p.C, 64, kKB, true);
+  else
+    rc = make_map(&mb, p.B, 1, p.ldb, p.C, 1, p.ldb, p.ldb * p.C, kHalf, kKB, false);
+  if (rc) return rc;
+  if (p.r > 0) {
+    const int half = split_half(p.r);
+    if ((rc = make_map(&mt, p.split, 2, 2 * half, p.M, 1, 4 * half, 4 * half * p.M, 64, kHalf,
+                       true)))
+      return rc;
+    if (MODE == kWideForward)
+      rc = make_map(&mbi, p.Bi, 2, p.r, p.N, p.E, p.ldbi * 2, p.ldbi * 2 * p.N, 64, kHalf, true);
+    else
+      rc = make_map(&mbi, p.Bi, 2, p.N, p.r, p.E, p.ldbi * 2, p.ldbi * 2 * p.r, 64, 64, true);
+    if (rc) return rc;
+  }
+  auto kern = k_wide<MODE>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+  if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(k_wide)", e);
+  const int items = g.tiles_m * g.tiles_n * g.splits;
+  const int units = device_sm_count(dev) / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (items < units ? items : units)));
+  cfg.blockDim = dim3(Cfg::THREADS);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.early ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, ma, mb, mt, mbi, g);
+  return e == cudaSuccess ? OZK_OK : set_cuda_error("k_wide launch", e);
+}
+
+}  // namespace
+
+size_t wide_partial_bytes(int64_t M, int64_t N, int64_t C, int dev) {
+  const int s = wide_splits(M, N, C, dev);
+  return s > 1 ? (size_t)s * M * N * 4 : 0;
+}
+
+int launch_wide(const WideProduct& p, int dev, cudaStream_t stream) {
+  WideArgs g = {};
+  g.M = p.M;
+  g.N = p.N;
+  g.C = p.C;
+  g.nkb = (int)((p.C + kKB - 1) / kKB);
+  const int64_t tm = (p.M + kTile - 1) / kTile, tn = (p.N + kTile - 1) / kTile;
+  if (tm * tn > (1 << 26)) return set_error(OZK_ERR_UNSUPPORTED, "too many output tiles");
+  g.tiles_m = (int)tm;
+  g.tiles_n = (int)tn;
+  g.group_m = 8;
+  g.splits = p.mode == kWideWeight && p.partial ? wide_splits(p.M, p.N, p.C, dev) : 1;
+  g.bf16 = p.bf16;
+  g.out_f32 = p.out_f32;
+  g.accumulate = p.accumulate;
+  g.out = p.out;
+  g.ldo = p.ldo;
+  g.o_vec = ((uintptr_t)p.out & 15) == 0 && p.ldo % (p.out_f32 ? 4 : 8) == 0;
+  g.partial = p.partial;
+  g.exps = p.exps;
+  g.ids = p.ids;
+  g.r = p.r;
+  g.E = p.E;
+  g.status = p.status;
+  g.budget_ns = wait_budget_ns();
+  int rc = p.mode == kWideForward ? launch_mode<kWideForward>(p, g, dev, stream)
+           : p.mode == kWideBack  ? launch_mode<kWideBack>(p, g, dev, stream)
+                                  : launch_mode<kWideWeight>(p, g, dev, stream);
+  if (rc || g.splits == 1) return rc;
+  int64_t blocks = (p.M * p.N + 255) / 256;
+  if (blocks > 148 * 8) blocks = 148 * 8;
+  k_wide_join<<<(unsigned)blocks, 256, 0, stream>>>(p.partial, g.splits, p.M, p.N, p.out, p.ldo,
+                                                    p.out_f32, p.bf16, p.accumulate);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? OZK_OK : set_cuda_error("k_wide_join launch", e);
+}
+
+}  // namespace ozk
