@@ -729,6 +729,29 @@ int run_linear(const Product& p, const int32_t* ids, const uint16_t* split, void
   g.budget_ns = wait_budget_ns();
   const int64_t tiles_m = (p.M + kRows - 1) / kRows;
   const int sms = device_sm_count(dev);
+  if (((p.M + 255) / 256) * ((p.n_out + 255) / 256) >= sms / 2) {
+    WideProduct w = {};
+    w.mode = p.back ? kWideBack : kWideForward;
+    w.bf16 = p.bf16;
+    w.M = p.M;
+    w.N = p.n_out;
+    w.C = p.n_in;
+    w.A = p.X.p;
+    w.lda = p.X.ld;
+    w.B = p.W.p;
+    w.ldb = p.W.ld;
+    w.ids = ids;
+    w.r = p.r;
+    w.E = p.E;
+    w.split = split;
+    w.Bi = p.B.p;
+    w.ldbi = p.B.ld;
+    w.early = true;
+    w.out = Y;
+    w.ldo = ldy;
+    w.status = status;
+    return launch_wide(w, dev, stream);
+  }
   const bool few = tiles_m * ((p.n_out + 127) / 128) < sms;
   const int64_t tiles = tiles_m * ((p.n_out + (few ? 63 : 127)) / (few ? 64 : 128));
   int splits = 1;

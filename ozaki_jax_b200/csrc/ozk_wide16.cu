@@ -12,12 +12,15 @@
 // MMAs of the next.
 //
 // Warps: 0 TMA producer, 1 MMA issuer (one thread of the even CTA), 2-5
-// epilogue, 6 the tile's list of adapters (forward, back) or 6-13 (weight)
-// the converters, which turn each CTA's 128 columns x 64 rows of codes (TMA'd
-// into a ring of their own) into 16-bit values in the MMA's layout: 16 codes
-// per clock and SM at the MMA's full rate, at about 2.5 instructions a code.
-// The exponents are powers of two, so a code times its step is exact in the
-// operand type and the product is that of the restored matrix.
+// epilogue, 6 the tile's list of adapters (forward, back) or 6-14 (weight):
+// 6-13 convert each CTA's 128 columns x 64 rows of codes (TMA'd into a ring of
+// their own) into 16-bit values in the MMA's layout, 16 codes per clock and SM
+// at the MMA's full rate, at about 2.5 instructions a code; two groups of four
+// warps take alternate stages, so that a group has two stages' time for its
+// chain of loads, conversions, stores and fence.  Warp 14 turns the exponents
+// into 16-bit steps and copies the codes in, some stages ahead of the MMA.  The steps are powers of two, so a code
+// times its step is exact in the operand type and the product is that of the
+// restored matrix.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -35,17 +38,17 @@ constexpr int kKB = 64;          // contraction indexes per stage
 constexpr int kABytes = kHalf * kKB * 2;
 constexpr int kStageBytes = 2 * kABytes;
 constexpr int kRawBytes = kHalf * kKB;
-constexpr int kConvWarps = 8;
+constexpr int kConvWarps = 4;    // of one of the two converter groups
 
 template <WideMode MODE>
 struct WideCfg {
   static constexpr bool W = MODE == kWideWeight;
   static constexpr int STAGES = W ? 5 : 6;
   static constexpr int RAW = W ? 6 : 0;
-  static constexpr int THREADS = W ? 32 * (6 + kConvWarps) : 32 * 7;
+  static constexpr int THREADS = W ? 32 * (7 + 2 * kConvWarps) : 32 * 7;
   // All of an SM's shared memory: a CTA holds all TMEM columns, so no other
   // TMEM kernel may share the SM.
-  static constexpr int SMEM = 227 * 1024 - (W ? 1024 : 11 * 1024);
+  static constexpr int SMEM = 227 * 1024 - (W ? 3 : 11) * 1024;
 };
 
 struct WideArgs {
@@ -128,7 +131,7 @@ __device__ __forceinline__ void store_row(const WideArgs& g, int64_t row, int64_
   }
 }
 
-template <WideMode MODE>
+template <WideMode MODE, bool BF16>
 __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
     k_wide(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
            const __grid_constant__ CUtensorMap mapT, const __grid_constant__ CUtensorMap mapBi,
@@ -142,6 +145,7 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
   __shared__ uint64_t full[STAGES], empty[STAGES], rfull[RAW + 1], rempty[RAW + 1], accf[2],
       acce[2], sfull, sempty, done;
   __shared__ SlotList<MODE == kWideWeight ? 1 : 8> slots;
+  __shared__ uint32_t steps[MODE == kWideWeight ? RAW : 1][kKB];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word;
   volatile int* s_abort = &s_abort_word;
@@ -159,7 +163,7 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < RAW; ++i) {
-      mbar_init(&rfull[i], 1);
+      mbar_init(&rfull[i], 2);  // the codes' bytes, the steps
       mbar_init(&rempty[i], kConvWarps);
     }
     for (int i = 0; i < 2; ++i) {
@@ -188,9 +192,9 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      Ring rg(STAGES), rr(RAW > 0 ? RAW : 1);
+      Ring rg(STAGES);
       bool ok = true, waited = false;
-      int issued = 0, raws = 0;
+      int issued = 0;
       uint32_t sph = 0;
       for (int i = unit; ok && i < items; i += n_units) {
         int tm, tn, sp, kb0, kb1;
@@ -220,19 +224,7 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
           ++issued;
           return true;
         };
-        for (int kb = kb0; ok && kb < kb1; ++kb) {
-          if constexpr (MODE == kWideWeight) {
-            if (!mbar_wait(&rempty[rr.s], rr.ph ^ 1, s_abort, g.status, g.budget_ns)) {
-              ok = false;
-              break;
-            }
-            mbar_arrive_expect_tx(&rfull[rr.s], kRawBytes);
-            tma_load_3d(sRaw + rr.s * kRawBytes, &mapB, &rfull[rr.s], bcol, kb * kKB, 0);
-            rr.next();
-            ++raws;
-          }
-          ok = load(&mapA, kb * kKB, &mapB, kb * kKB, 0);
-        }
+        for (int kb = kb0; ok && kb < kb1; ++kb) ok = load(&mapA, kb * kKB, &mapB, kb * kKB, 0);
         if (MODE != kWideWeight && g.r > 0) {
           if (!waited) grid_wait();  // the split T comes from the kernel before this one
           waited = true;
@@ -254,14 +246,11 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
         for (int i = 0; i < issued; ++i, b.next())
           if (i >= issued - STAGES) mbar_wait(&full[b.s], b.ph, nullptr, g.status, g.budget_ns);
       }
-      Ring b(RAW > 0 ? RAW : 1);
-      for (int i = 0; i < raws; ++i, b.next())
-        if (i >= raws - RAW) mbar_wait(&rfull[b.s], b.ph, nullptr, g.status, g.budget_ns);
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = umma_idesc_16(g.bf16, kTile, kTile, AMN, BMN);
+      const uint32_t idesc = umma_idesc_16(BF16, kTile, kTile, AMN, BMN);
       Ring rg(STAGES);
       bool ok = true;
       int it = 0;
@@ -282,7 +271,7 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
         const uint32_t d = tmem + buf * kTile;
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = MODE == kWideWeight
-                   ? mbar_wait_cluster(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns)
+                   ? mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns)
                    : mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
           if (!ok) break;
           tc_fence_after();
@@ -374,60 +363,96 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
       }
     }
   } else if constexpr (MODE == kWideWeight) {
-    // ------------------------------------------------------------ converters
-    // Thread: rows t / 16 + 16 j of the stage, 8 columns at 8 (t % 16); lanes of
-    // a half warp write one row's 16-byte pieces, eight to a 128-byte line.
-    const int t = threadIdx.x - 192;
-    const int piece = t & 15, r0 = t >> 4;
-    const uint32_t to = smem_u32(smem) + kABytes + (piece >> 3) * 8192;
-    Ring rg(STAGES), rr(RAW);
-    bool ok = true;
-    for (int i = unit; ok && i < items; i += n_units) {
-      int tm, tn, sp, kb0, kb1;
-      item_at(i, tm, tn, sp, kb0, kb1);
-      const int64_t group = (int64_t)tn * 2 + rank;
-      const bool inside = group * kGroup < g.N;
-      const int8_t* ex = g.exps + (inside ? group * g.C : 0);
-      auto exp_of = [&](int kb, int j) {
-        const int64_t m = (int64_t)kb * kKB + r0 + 16 * j;
-        return inside && m < g.C ? (int)__ldg(ex + m) : -127;
-      };
-      int e[4];
+    if (warp == 6 + 2 * kConvWarps) {
+      // ------------------------------------------- codes' copies and steps
+      Ring rr(RAW);
+      bool ok = true;
+      int raws = 0;
+      for (int i = unit; ok && i < items; i += n_units) {
+        int tm, tn, sp, kb0, kb1;
+        item_at(i, tm, tn, sp, kb0, kb1);
+        const int64_t group = (int64_t)tn * 2 + rank;
+        const bool inside = group * kGroup < g.N;
+        const int8_t* ex = g.exps + (inside ? group * g.C : 0);
+        constexpr int AHEAD = 4;  // stages whose exponents are in flight
+        int e[AHEAD][2];
+        auto fetch = [&](int kb, int (&v)[2]) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = exp_of(kb0, j);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        int en[4];
+          for (int h = 0; h < 2; ++h) {
+            const int64_t m = (int64_t)kb * kKB + h * 32 + lane;
+            v[h] = inside && kb < kb1 && m < g.C ? (int)__ldg(ex + m) : 0;
+          }
+        };
 #pragma unroll
-        for (int j = 0; j < 4; ++j) en[j] = kb + 1 < kb1 ? exp_of(kb + 1, j) : 0;
-        ok = mbar_wait(&rfull[rr.s], rr.ph, s_abort, g.status, g.budget_ns);
-        if (!ok) break;
-        uint2 q[4];
+        for (int a = 0; a < AHEAD; ++a) fetch(kb0 + a, e[a]);
+        for (int kb = kb0; ok && kb < kb1; kb += AHEAD) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          q[j] = *(const uint2*)(sRaw + rr.s * kRawBytes + (r0 + 16 * j) * kHalf + piece * 8);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&rempty[rr.s]);
-        ok = mbar_wait(&empty[rg.s], rg.ph ^ 1, s_abort, g.status, g.budget_ns);
-        if (!ok) break;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = r0 + 16 * j;
-          const uint32_t sc = exp_pair(g.bf16, e[j]);
-          uint32_t w[4];
-          codes_to_16(g.bf16, q[j].x, sc, w[0], w[1]);
-          codes_to_16(g.bf16, q[j].y, sc, w[2], w[3]);
-          const uint32_t at = to + rg.s * kStageBytes + row * 128 +
-                              (((uint32_t)(piece & 7) ^ (uint32_t)(row & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
-                       "r"(w[2]), "r"(w[3])
-                       : "memory");
-          e[j] = en[j];
+          for (int a = 0; a < AHEAD; ++a) {
+            if (kb + a >= kb1) break;
+            ok = mbar_wait(&rempty[rr.s], rr.ph ^ 1, s_abort, g.status, g.budget_ns);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&rfull[rr.s], kRawBytes);
+              tma_load_3d(sRaw + rr.s * kRawBytes, &mapB, &rfull[rr.s],
+                          tn * kTile + (int)rank * kHalf, (kb + a) * kKB, 0);
+            }
+            ++raws;
+            steps[rr.s][lane] = exp_pair(BF16, e[a][0]);
+            steps[rr.s][lane + 32] = exp_pair(BF16, e[a][1]);
+            fetch(kb + a + AHEAD, e[a]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&rfull[rr.s]);
+            rr.next();
+          }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_u32(&full[rg.s], 0));
-        rg.next();
-        rr.next();
+      }
+      Ring b(RAW);
+      for (int i = 0; i < raws; ++i, b.next())
+        if (i >= raws - RAW) mbar_wait(&rfull[b.s], b.ph, nullptr, g.status, g.budget_ns);
+    } else {
+      // ---------------------------------------------------------- converters
+      // Thread: rows t / 16 + 8 j of the stage, 8 columns at 8 (t % 16); lanes
+      // of a half warp write one row's 16-byte pieces, eight to a 128-byte line.
+      const int cg = (warp - 6) / kConvWarps;  // converter group
+      const int t = (threadIdx.x - 192) % (32 * kConvWarps);
+      const int piece = t & 15, r0 = t >> 4;
+      const uint32_t to = smem_u32(smem) + kABytes + (piece >> 3) * 8192;
+      Ring rg(STAGES), rr(RAW);
+      bool ok = true;
+      int turn = 0;
+      for (int i = unit; ok && i < items; i += n_units) {
+        int tm, tn, sp, kb0, kb1;
+        item_at(i, tm, tn, sp, kb0, kb1);
+        for (int kb = kb0; kb < kb1; ++kb, turn ^= 1, rg.next(), rr.next()) {
+          if (turn != cg) continue;
+          ok = mbar_wait(&rfull[rr.s], rr.ph, s_abort, g.status, g.budget_ns);
+          if (!ok) break;
+          uint2 q[8];
+          uint32_t sc[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            q[j] = *(const uint2*)(sRaw + rr.s * kRawBytes + (r0 + 8 * j) * kHalf + piece * 8);
+            sc[j] = steps[rr.s][r0 + 8 * j];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&rempty[rr.s]);
+          ok = mbar_wait(&empty[rg.s], rg.ph ^ 1, s_abort, g.status, g.budget_ns);
+          if (!ok) break;
+          const uint32_t at0 = to + rg.s * kStageBytes + r0 * 128 +
+                               (((uint32_t)(piece & 7) ^ (uint32_t)(r0 & 7)) << 4);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];
+            codes_to_16(BF16, q[j].x, sc[j], w[0], w[1]);
+            codes_to_16(BF16, q[j].y, sc[j], w[2], w[3]);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at0 + j * 1024), "r"(w[0]),
+                         "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(mapa_u32(&full[rg.s], 0));
+        }
       }
     }
   } else {
@@ -511,7 +536,7 @@ int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) 
       rc = make_map(&mbi, p.Bi, 2, p.N, p.r, p.E, p.ldbi * 2, p.ldbi * 2 * p.r, 64, 64, true);
     if (rc) return rc;
   }
-  auto kern = k_wide<MODE>;
+  auto kern = p.bf16 ? k_wide<MODE, true> : k_wide<MODE, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
   if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(k_wide)", e);
   const int items = g.tiles_m * g.tiles_n * g.splits;
