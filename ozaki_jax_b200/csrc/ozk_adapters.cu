@@ -170,10 +170,7 @@ __global__ void __launch_bounds__(kThreads)
           ok = load(&mapT, ax, &mapB, blocks == 1 ? 0 : (b >> 1) * 64, slots.id[j]);
         }
       // Every copy lands before the shared memory is reused or released.
-      Ring back(g.stages);
-      for (int i = 0; i < issued; ++i, back.next())
-        if (i >= issued - g.stages)
-          mbar_wait(&full[back.s], back.ph, nullptr, g.status, g.budget_ns);
+      ring_drain(full, g.stages, issued, g.status, g.budget_ns);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -398,11 +395,8 @@ __global__ void __launch_bounds__(kThreads)
           ++ia;
         }
       }
-      Ring bx(g.xstages), ba(g.astages);
-      for (int i = 0; i < ix; ++i, bx.next())
-        if (i >= ix - g.xstages) mbar_wait(&xfull[bx.s], bx.ph, nullptr, g.status, g.budget_ns);
-      for (int i = 0; i < ia; ++i, ba.next())
-        if (i >= ia - g.astages) mbar_wait(&afull[ba.s], ba.ph, nullptr, g.status, g.budget_ns);
+      ring_drain(xfull, g.xstages, ix, g.status, g.budget_ns);
+      ring_drain(afull, g.astages, ia, g.status, g.budget_ns);
     }
     __syncwarp();
   } else if (warp == 1) {

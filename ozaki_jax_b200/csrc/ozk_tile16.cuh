@@ -105,6 +105,7 @@ struct Ring {
   int s = 0;
   uint32_t ph = 0;
   __device__ explicit Ring(int stages) : n(stages) {}
+  __device__ Ring(int stages, int step) : n(stages), s(step % stages), ph((step / stages) & 1) {}
   __device__ void next() {
     if (++s == n) {
       s = 0;
@@ -112,6 +113,16 @@ struct Ring {
     }
   }
 };
+
+// Waits for the last copies of a ring that has run `steps` steps, so that its
+// shared memory may be reused or released.
+__device__ __forceinline__ void ring_drain(uint64_t* full, int stages, int steps, int32_t* status,
+                                           uint64_t budget_ns) {
+  const int first = steps > stages ? steps - stages : 0;
+  Ring b(stages, first);
+  for (int i = first; i < steps; ++i, b.next())
+    mbar_wait(&full[b.s], b.ph, nullptr, status, budget_ns);
+}
 
 // Columns of the split T of rank r, high or low half: 32 up to rank 32, else
 // ceil(r / 64) blocks of 64.

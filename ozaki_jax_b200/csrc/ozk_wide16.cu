@@ -241,11 +241,7 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
       if (!waited) grid_wait();
       // Drain: every copy lands before shared memory is released (the even
       // CTA's full barriers count both CTAs' bytes).
-      if (rank == 0) {
-        Ring b(STAGES);
-        for (int i = 0; i < issued; ++i, b.next())
-          if (i >= issued - STAGES) mbar_wait(&full[b.s], b.ph, nullptr, g.status, g.budget_ns);
-      }
+      if (rank == 0) ring_drain(full, STAGES, issued, g.status, g.budget_ns);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -270,9 +266,7 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
         tc_fence_after();
         const uint32_t d = tmem + buf * kTile;
         for (int kb = kb0; kb < kb1; ++kb) {
-          ok = MODE == kWideWeight
-                   ? mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns)
-                   : mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
+          ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
           if (!ok) break;
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + rg.s * kStageBytes), b0 = a0 + kABytes;
@@ -406,9 +400,7 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
           }
         }
       }
-      Ring b(RAW);
-      for (int i = 0; i < raws; ++i, b.next())
-        if (i >= raws - RAW) mbar_wait(&rfull[b.s], b.ph, nullptr, g.status, g.budget_ns);
+      ring_drain(rfull, RAW, raws, g.status, g.budget_ns);
     } else {
       // ---------------------------------------------------------- converters
       // Thread: rows t / 16 + 8 j of the stage, 8 columns at 8 (t % 16); lanes
