@@ -447,6 +447,20 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
                         int E, int dt, void* workspace, size_t ws_bytes, int32_t* status_dev,
                         void* stream);
 
+/* Gradients of ozk_matmul_adapters, W being fixed:
+ *   U = alpha scale[i] dY B_i, dX = dY W + U A_i (skipped when dX is NULL),
+ *   dA_i = sum of U_m^T X_m and dB_i = sum of dY_m^T T_m over adapter i's rows
+ *   (0 for an adapter without rows).
+ * X: [M][K] (ldx) of type dt, or, with exps set, the int8 codes of
+ * ozk_checkpoint_rows made from type dt (ldx = K rounded up to 128).  T: FP32
+ * [M][r], the `low` of the forward call.  dX [M][K] (lddx), dA [E][r][K] and
+ * dB [E][N][r] of type dt.  Sums over rows are FP32 in a fixed order. */
+size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E);
+int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, const void* exps,
+                      const void* W, int64_t ldw, const void* A, const void* B, const int32_t* ids,
+                      const float* T, const float* scale, double alpha, void* dX, int64_t lddx,
+                      void* dA, void* dB, int64_t M, int64_t N, int64_t K, int r, int E, int dt,
+                      void* workspace, size_t ws_bytes, int32_t* status_dev, void* stream);
 /* Rows of X [M][K] (ldx, type dt: any OZK_DT_*) as int8 codes and exponents.
  * A group of 128 columns of a row shares the step 2^e, the smallest power of
  * two under which its largest magnitude rounds to at most 127;

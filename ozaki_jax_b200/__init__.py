@@ -18,7 +18,7 @@ from .extract import (
     f32_extract_split_rows, f32_extract_split_cols,
     jax_extract_split_rows, jax_extract_split_cols,
 )
-from .adapters import matmul_adapters
+from .adapters import matmul_adapters, adapters_grad
 from .checkpoint import SavedRows, checkpoint_rows, restore_rows, checkpoint_grad
 from .accum import accumulate_2sum, validate_accumulation_2sum
 
@@ -28,7 +28,7 @@ __all__ = [
     "f32_extract_split_rows", "f32_extract_split_cols",
     "jax_extract_split_rows", "jax_extract_split_cols",
     "SavedRows", "checkpoint_rows", "restore_rows", "checkpoint_grad",
-    "matmul_adapters",
+    "matmul_adapters", "adapters_grad",
     "accumulate_2sum", "validate_accumulation_2sum",
     "compute_rho_f32", "compute_rho_f64", "ondevice_safety_report",
 ]

@@ -136,3 +136,51 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
     elif low is not None:
         low.zero_()
     return (Y, low) if return_low else Y
+
+
+def adapters_grad(dY, X, W, A, B, ids, T, scale=1.0, input_grad=True):
+    """Gradients of Y = matmul_adapters(X, W, A, B, ids, scale) for the
+    gradient dY (M, N) of Y, W being fixed:
+
+        U  = scale[i] dY B_i
+        dX = dY W + U A_i
+        dA_i, dB_i = sums of U_m^T X_m and dY_m^T T_m over adapter i's rows
+
+    X is the layer's input (M, K), or its SavedRows.  T is what the forward
+    call returned beside Y.  Returns (dX, dA, dB) in the type of dY, dX None
+    without input_grad; adapters without rows get zeros.
+    """
+    from .checkpoint import SavedRows
+    check_16bit("dY", dY)
+    M = dY.shape[0]
+    N, K, E, r = _adapter_shapes(W, A, B, ids, scale, M, dY.dtype)
+    check_matrix("dY", dY, cols=N)
+    dev = dY.device
+    factors, alpha = _scale_args(scale)
+    if isinstance(X, SavedRows):
+        if X.dtype != dY.dtype:
+            raise ValueError(f"X was saved from {X.dtype}, expected {dY.dtype}.")
+        if tuple(X.shape) != (M, K):
+            raise ValueError(f"X has shape {tuple(X.shape)}, expected {(M, K)}.")
+        Xd, exps, ldx = X.codes, X.exps, X.codes.shape[1]
+    else:
+        check_matrix("X", X, dY.dtype, rows=M, cols=K)
+        Xd, ldx = row_major(X)
+        exps = None
+    check_matrix("T", T, torch.float32, rows=M, cols=r)
+    check_device(dev, X=Xd, W=W, A=A, B=B, ids=ids, T=T, scale=factors)
+    (dY, ldy), (W, ldw) = row_major(dY), row_major(W)
+    A, B, T = A.contiguous(), B.contiguous(), T.contiguous()
+    ids = None if ids is None else ids.contiguous()
+    dX = torch.empty((M, K), dtype=dY.dtype, device=dev) if input_grad else None
+    dA, dB = torch.empty_like(A), torch.empty_like(B)
+    lib = L.load()
+    with D.on_device(dev):
+        n = lib.ozk_adapters_grad_workspace_bytes(M, N, K, r, E)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        L.check(lib.ozk_adapters_grad(
+            dY.data_ptr(), ldy, Xd.data_ptr(), ldx, _ptr(exps), W.data_ptr(), ldw, A.data_ptr(),
+            B.data_ptr(), _ptr(ids), T.data_ptr(), _ptr(factors), alpha, _ptr(dX), K,
+            dA.data_ptr(), dB.data_ptr(), M, N, K, r, E, DTYPES[dY.dtype], ws.data_ptr(), n, None,
+            D.stream_handle(dev)))
+    return dX, dA, dB

@@ -26,6 +26,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include "ozk_adapters.h"
 #include "ozk_tile16.cuh"
 
 namespace ozk {
@@ -837,6 +838,85 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
   }
   if ((rc = run_low_rank(p, ids, scale, (float)alpha, low, split, status_dev, dev, s))) return rc;
   return run_linear(p, ids, split, Y, ldy, status_dev, dev, s);
+}
+
+size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E) {
+  if (M < 1 || N < 1 || K < 1 || r < 1 || r > kMaxRank || E < 1) return 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  Arena ws(nullptr);
+  ws.take((size_t)M * 4 * split_half(r));
+  ws.take((size_t)M * r * 4);
+  ws.take(outer_scratch_bytes(M, N, K, r, E, dev));
+  ws.take((size_t)M * round_up(N, 8) * 2);
+  ws.take((size_t)N * round_up(K, 8) * 2);
+  ws.take((size_t)E * r * round_up(K, 8) * 2);
+  ws.take((size_t)E * N * round_up(r, 8) * 2);
+  return ws.used;
+}
+
+int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, const void* exps,
+                      const void* W, int64_t ldw, const void* A, const void* B, const int32_t* ids,
+                      const float* T, const float* scale, double alpha, void* dX, int64_t lddx,
+                      void* dA, void* dB, int64_t M, int64_t N, int64_t K, int r, int E, int dt,
+                      void* workspace, size_t ws_bytes, int32_t* status_dev, void* stream) {
+  int rc = adapter_args(X, ldx, W, ldw, A, B, M, N, K, r, E, dt);
+  if (rc) return rc;
+  if (E > 65535) return set_error(OZK_ERR_UNSUPPORTED, "at most 65535 adapters");
+  if (!dA || (N && !dB)) return set_error(OZK_ERR_ARG, "NULL dA or dB");
+  cudaStream_t s = (cudaStream_t)stream;
+  if (M == 0 || N == 0) {
+    // No rows or no outputs: the gradients are zero.
+    cudaError_t e = cudaMemsetAsync(dA, 0, (size_t)E * r * K * 2, s);
+    if (e == cudaSuccess && N) e = cudaMemsetAsync(dB, 0, (size_t)E * N * r * 2, s);
+    if (e == cudaSuccess && M && dX)
+      e = cudaMemset2DAsync(dX, (size_t)lddx * 2, 0, (size_t)K * 2, (size_t)M, s);
+    return e == cudaSuccess ? OZK_OK : set_cuda_error("cudaMemsetAsync", e);
+  }
+  if (!dY || !T || ldy < N) return set_error(OZK_ERR_ARG, "NULL dY or T, or ldy < N");
+  if (exps ? (ldx != round_up(K, kGroup) || ((uintptr_t)X & 15)) : ldx < K)
+    return set_error(OZK_ERR_ARG, exps ? "codes need 16 bytes of alignment and ldx = K rounded up to 128"
+                                       : "ldx < K");
+  if (dX && lddx < K) return set_error(OZK_ERR_ARG, "lddx < K");
+  int dev;
+  cudaGetDevice(&dev);
+  Product p = {{dY, ldy}, {W, ldw}, {B, r}, {A, K}, M, K, N, r, E, true, dt == OZK_DT_BF16};
+  Arena ws(workspace);
+  uint16_t* split = ws.take<uint16_t>((size_t)M * 4 * split_half(r));
+  float* U = ws.take<float>((size_t)M * r * 4);
+  void* scratch = ws.take(outer_scratch_bytes(M, N, K, r, E, dev));
+  for (int pass = 0; pass < 2; ++pass) {
+    Product q = p;
+    Arena w = ws;
+    if ((rc = align_operand(q.X, M, N, w, pass, s)) || (rc = align_operand(q.W, N, K, w, pass, s)) ||
+        (rc = align_operand(q.A, (int64_t)E * N, r, w, pass, s)) ||
+        (rc = align_operand(q.B, (int64_t)E * r, K, w, pass, s)))
+      return rc;
+    if (pass) p = q;
+    else if (!workspace || w.used > ws_bytes || ((uintptr_t)workspace & 127))
+      return set_error(OZK_ERR_WORKSPACE, "workspace of %zu bytes, aligned to 128, needed", w.used);
+  }
+  if ((rc = run_low_rank(p, ids, scale, (float)alpha, U, split, status_dev, dev, s))) return rc;
+  if (dX && (rc = run_linear(p, ids, split, dX, lddx, status_dev, dev, s))) return rc;
+  OuterProduct o = {};
+  o.bf16 = p.bf16;
+  o.M = M;
+  o.N = N;
+  o.K = K;
+  o.r = r;
+  o.E = E;
+  o.ids = ids;
+  o.X = X;
+  o.ldx = ldx;
+  o.exps = (const int8_t*)exps;
+  o.dY = p.X.p;
+  o.ldy = p.X.ld;
+  o.U = U;
+  o.T = T;
+  o.dA = dA;
+  o.dB = dB;
+  o.status = status_dev;
+  return launch_outer(o, scratch, dev, s);
 }
 
 }  // extern "C"

@@ -1,0 +1,27 @@
+// The adapters' own gradients (ozk_adapters_grad.cu), as ozk_adapters_grad calls them.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ozk {
+
+struct OuterProduct {
+  bool bf16;
+  int64_t M, N, K;
+  int r, E;
+  const int32_t* ids;
+  const void* X;        // 16-bit [M][K], or int8 codes when exps is set
+  int64_t ldx;
+  const int8_t* exps;
+  const void* dY;       // [M][N]
+  int64_t ldy;
+  const float *U, *T;   // [M][r]
+  void *dA, *dB;        // [E][r][K], [E][N][r]
+  int32_t* status;
+};
+
+size_t outer_scratch_bytes(int64_t M, int64_t N, int64_t K, int r, int E, int dev);
+int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t stream);
+
+}  // namespace ozk
