@@ -429,6 +429,11 @@ int ozk_set_l2_persisting(size_t bytes, size_t* previous);
 #define OZK_DT_F16 1
 #define OZK_DT_F32 2
 
+/* The current device's status word (int32 in page-locked host memory that the
+ * device can write, made on first use, also during a stream capture): a
+ * status_dev for calls that nobody waits for.  The host may read it at any
+ * time and sets it back to 0. */
+int ozk_status_word(int32_t** word);
 /* Y = X W^T + T B_i^T with T = alpha scale[i] X A_i^T, i = ids[row].
  *   X [M][K] (ldx), W [N][K] (ldw), A [E][r][K], B [E][N][r], all of type dt
  *   (OZK_DT_BF16 or OZK_DT_F16); A and B contiguous.
@@ -439,8 +444,10 @@ int ozk_set_l2_persisting(size_t bytes, size_t* previous);
  * Sums are FP32; T enters the second product as the sum of two 16-bit values
  * (with OZK_DT_F16, |T| must stay below 65504).  1 <= r <= 128.  Nothing may
  * alias Y or low.  Operands whose base or row stride is not a multiple of 16
- * bytes are copied into the workspace first. */
-size_t ozk_matmul_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E);
+ * bytes are copied into the workspace first; a workspace asked for with
+ * `aligned` set has no room for that. */
+size_t ozk_matmul_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E,
+                                         int aligned);
 int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* A,
                         const void* B, const int32_t* ids, const float* scale, double alpha,
                         void* Y, int64_t ldy, float* low, int64_t M, int64_t N, int64_t K, int r,
@@ -455,7 +462,8 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
  * ozk_checkpoint_rows made from type dt (ldx = K rounded up to 128).  T: FP32
  * [M][r], the `low` of the forward call.  dX [M][K] (lddx), dA [E][r][K] and
  * dB [E][N][r] of type dt.  Sums over rows are FP32 in a fixed order. */
-size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E);
+size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E,
+                                         int aligned);
 int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, const void* exps,
                       const void* W, int64_t ldw, const void* A, const void* B, const int32_t* ids,
                       const float* T, const float* scale, double alpha, void* dX, int64_t lddx,
@@ -480,7 +488,7 @@ int ozk_restore_rows(const void* codes, int64_t ldc, const void* exps, int64_t M
  * the restored rows, out [N][K] (ldo) of type out_dt (dt or OZK_DT_F32).  FP32
  * sums, one rounding.  The result does not depend on scheduling: where the
  * rows are split, the parts are added in order. */
-size_t ozk_checkpoint_grad_workspace_bytes(int64_t M, int64_t N, int64_t K);
+size_t ozk_checkpoint_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int aligned);
 int ozk_checkpoint_grad(const void* dY, int64_t ldy, const void* codes, int64_t ldc,
                         const void* exps, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
                         int dt, int out_dt, int accumulate, void* workspace, size_t ws_bytes,

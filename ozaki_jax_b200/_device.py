@@ -73,8 +73,40 @@ def to_host_f64(t):
     return t.cpu().numpy()
 
 
+# The raw handle without a Stream object around it, where torch has the call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device):
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_status = {}
+
+
+def status_word(device):
+    """Address of the device's status word for calls that do not wait for
+    their kernels: page-locked host memory that a kernel whose bounded wait
+    ran out writes to.  A word that is set raises here, in the next call."""
+    word = _status.get(device.index)
+    if word is None:
+        import ctypes
+
+        from . import _lib as L
+        address = ctypes.c_void_p()
+        with on_device(device):
+            L.check(L.load().ozk_status_word(ctypes.byref(address)))
+        word = _status[device.index] = ctypes.c_int32.from_address(address.value)
+        word.address = address.value
+    if word.value:
+        from . import _lib as L
+        flags, word.value = word.value, 0
+        raise L.OzakiError(L.OZK_ERR_TIMEOUT,
+                           f"an earlier call's kernel gave up a wait (flags {flags:#x}); its "
+                           "results are not valid")
+    return word.address
 
 
 class _Here:

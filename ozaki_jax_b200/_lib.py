@@ -105,16 +105,17 @@ SIGNATURES = {
     "ozk_residual_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int, c_int]),
     "ozk_residual_f64": (c_int, [vp, c_i64, vp, c_i64, vp, c_i64, vp, c_i64, c_i64, c_i64, c_i64,
                                  c_int, c_int, c_int, vp, c_size, vp, vp]),
-    "ozk_matmul_adapters_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int, c_int]),
+    "ozk_status_word": (c_int, [vp]),
+    "ozk_matmul_adapters_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int, c_int, c_int]),
     "ozk_matmul_adapters": (c_int, [vp, c_i64, vp, c_i64, vp, vp, vp, vp, c_dbl, vp, c_i64, vp,
                                     c_i64, c_i64, c_i64, c_int, c_int, c_int, vp, c_size, vp, vp]),
-    "ozk_adapters_grad_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int, c_int]),
+    "ozk_adapters_grad_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int, c_int, c_int]),
     "ozk_adapters_grad": (c_int, [vp, c_i64, vp, c_i64, vp, vp, c_i64, vp, vp, vp, vp, vp, c_dbl,
                                   vp, c_i64, vp, vp, c_i64, c_i64, c_i64, c_int, c_int, c_int, vp,
                                   c_size, vp, vp]),
     "ozk_checkpoint_rows": (c_int, [vp, c_i64, c_i64, c_i64, c_int, vp, c_i64, vp, vp]),
     "ozk_restore_rows": (c_int, [vp, c_i64, vp, c_i64, c_i64, vp, c_i64, c_int, vp]),
-    "ozk_checkpoint_grad_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
+    "ozk_checkpoint_grad_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_int]),
     "ozk_checkpoint_grad": (c_int, [vp, c_i64, vp, c_i64, vp, vp, c_i64, c_i64, c_i64, c_i64,
                                     c_int, c_int, c_int, vp, c_size, vp, vp]),
     "ozk_check_status": (c_int, [vp, vp]),

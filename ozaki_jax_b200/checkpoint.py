@@ -12,7 +12,7 @@ import torch
 
 from . import _device as D
 from . import _lib as L
-from .adapters import DTYPES, check_16bit, check_device, check_matrix, row_major
+from ._checks import DTYPES, check_16bit, check_device, check_matrix, row_major
 
 GROUP = 128
 
@@ -40,7 +40,7 @@ class SavedRows:
         if tuple(exps.shape) != (groups, codes.shape[0]):
             raise ValueError(f"exps has shape {tuple(exps.shape)}, expected "
                              f"{(groups, codes.shape[0])}.")
-        if exps.device != codes.device:
+        if exps.get_device() != codes.get_device():
             raise ValueError(f"exps is on {exps.device}, expected {codes.device}.")
         if not codes.is_contiguous() or not exps.is_contiguous():
             raise ValueError("codes and exps must be contiguous.")
@@ -67,23 +67,22 @@ class SavedRows:
 def checkpoint_rows(X):
     """The rows of a CUDA tensor X (M, K), bfloat16, float16 or float32, as
     SavedRows: about half the bytes of a 16-bit X, a quarter of a float32 one."""
-    check_matrix("X", X)
-    if X.dtype not in DTYPES:
-        raise ValueError(f"X must be bfloat16, float16 or float32, got {X.dtype}.")
-    M, K = X.shape
+    M, K = check_matrix("X", X)
+    dtype = X.dtype
+    if dtype not in DTYPES:
+        raise ValueError(f"X must be bfloat16, float16 or float32, got {dtype}.")
     if K < 1:
         raise ValueError("X has no columns.")
-    dev = X.device
-    check_device(dev)
+    dev = check_device(X)
     X, ldx = row_major(X)
     groups = (K + GROUP - 1) // GROUP
     codes = torch.empty((M, groups * GROUP), dtype=torch.int8, device=dev)
     exps = torch.empty((groups, M), dtype=torch.int8, device=dev)
     with D.on_device(dev):
-        L.check(L.load().ozk_checkpoint_rows(X.data_ptr(), ldx, M, K, DTYPES[X.dtype],
+        L.check(L.load().ozk_checkpoint_rows(X.data_ptr(), ldx, M, K, DTYPES[dtype],
                                              codes.data_ptr(), groups * GROUP, exps.data_ptr(),
                                              D.stream_handle(dev)))
-    return SavedRows(codes, exps, K, X.dtype)
+    return SavedRows(codes, exps, K, dtype)
 
 
 def restore_rows(saved, dtype=None):
@@ -93,8 +92,7 @@ def restore_rows(saved, dtype=None):
     dtype = saved.dtype if dtype is None else dtype
     if dtype not in (saved.dtype, torch.float32):
         raise ValueError(f"dtype={dtype}; expected {saved.dtype} or float32.")
-    dev = saved.device
-    check_device(dev)
+    dev = check_device(saved.codes)
     M, K = saved.shape
     out = torch.empty((M, K), dtype=dtype, device=dev)
     with D.on_device(dev):
@@ -113,38 +111,39 @@ def checkpoint_grad(dY, saved, out=None, accumulate=False, dtype=None):
     if given (its rows may be strided), and with accumulate it is added to
     what `out` holds.  FP32 sums, rounded once.
     """
-    check_16bit("dY", dY)
+    (M, N), dtype_y = check_16bit("dY", dY)
     if not isinstance(saved, SavedRows):
         raise ValueError(f"saved must be SavedRows, got {type(saved).__name__}.")
-    M, K = saved.shape
-    check_matrix("dY", dY, saved.dtype, rows=M)
-    N = dY.shape[1]
-    dev = dY.device
-    check_device(dev, saved=saved.codes)
+    K = saved.cols
+    if dtype_y is not saved.dtype:
+        raise ValueError(f"dY must be {saved.dtype}, got {dtype_y}.")
+    if M != saved.codes.shape[0]:
+        raise ValueError(f"dY has {M} rows, expected {saved.codes.shape[0]}.")
+    dev = check_device(dY, saved.codes, out)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out.")
-        dtype = dY.dtype if dtype is None else dtype
-        if dtype not in (dY.dtype, torch.float32):
-            raise ValueError(f"dtype={dtype}; expected {dY.dtype} or float32.")
+        dtype = dtype_y if dtype is None else dtype
+        if dtype not in (dtype_y, torch.float32):
+            raise ValueError(f"dtype={dtype}; expected {dtype_y} or float32.")
         out = torch.empty((N, K), dtype=dtype, device=dev)
     else:
         check_matrix("out", out, rows=N, cols=K)
-        if out.dtype not in (dY.dtype, torch.float32):
-            raise ValueError(f"out must be {dY.dtype} or float32, got {out.dtype}.")
+        if out.dtype not in (dtype_y, torch.float32):
+            raise ValueError(f"out must be {dtype_y} or float32, got {out.dtype}.")
         if dtype is not None and dtype != out.dtype:
             raise ValueError(f"dtype={dtype}, but out is {out.dtype}.")
         if (K > 1 and out.stride(1) != 1) or (N > 1 and out.stride(0) < K):
             raise ValueError("out must be row-major with rows that do not overlap.")
-        check_device(dev, out=out)
     dY, ldy = row_major(dY)
     lib = L.load()
+    y = dY.data_ptr()
     with D.on_device(dev):
-        n = lib.ozk_checkpoint_grad_workspace_bytes(M, N, K)
+        n = lib.ozk_checkpoint_grad_workspace_bytes(M, N, K, not (y & 15 or ldy & 7))
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         L.check(lib.ozk_checkpoint_grad(
-            dY.data_ptr(), ldy, saved.codes.data_ptr(), saved.codes.shape[1],
+            y, ldy, saved.codes.data_ptr(), saved.codes.shape[1],
             saved.exps.data_ptr(), out.data_ptr(), out.stride(0) if N > 1 else K, M, N, K,
-            DTYPES[dY.dtype], DTYPES[out.dtype], int(accumulate), ws.data_ptr(), n, None,
-            D.stream_handle(dev)))
+            DTYPES[dtype_y], DTYPES[out.dtype], int(accumulate), ws.data_ptr(), n,
+            D.status_word(dev), D.stream_handle(dev)))
     return out

@@ -69,17 +69,24 @@ __device__ __forceinline__ void store_cols(void* Y, int64_t at, const uint32_t* 
   }
 }
 
-// Sum over the CTAs of the cluster, in rank order, of the FP32 partial at
-// shared-memory address `a` of each.
+// Sum over the CTAs of the cluster (at most 8), in rank order, of the FP32
+// partial at shared-memory address `a` of each.  The loads are independent, so
+// their round trips overlap.
 __device__ __forceinline__ float cluster_sum(uint32_t a, int splits) {
-  float s = 0.0f;
-  for (int q = 0; q < splits; ++q) {
-    uint32_t ra;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(q));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ra) : "memory");
-    s += v;
+  float v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    v[q] = 0.0f;
+    if (q < splits) {
+      uint32_t ra;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(q));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[q]) : "r"(ra) : "memory");
+    }
   }
+  float s = v[0];
+#pragma unroll
+  for (int q = 1; q < 8; ++q)
+    if (q < splits) s += v[q];
   return s;
 }
 
@@ -300,6 +307,7 @@ struct LowArgs {
   uint16_t* split;   // [M][2 half], or NULL
   int64_t M;
   int nkb, E, r, rp;  // rp: r rounded up to 16
+  int nacc;           // accumulators that the stages go to in turn
   int bf16;
   int xstages, astages, xrows;
   int32_t* status;
@@ -316,10 +324,15 @@ __device__ __forceinline__ void store_split(uint16_t* split, int64_t row, int ha
   split[row * 2 * half + half + c] = round16(bf16, rest);
 }
 
-// T of a tile of 128 rows: one accumulator of rp columns; each block of 64
-// contraction elements of X is loaded once and multiplied with the same block
-// of every adapter of the tile, each into its own lanes.  The CTAs of a
-// cluster split the contraction.  Bound by reading X.
+// T of a tile of 128 rows: each block of 64 contraction elements of X is loaded
+// once and multiplied with the same block of every adapter of the tile, each
+// into its own lanes.  The CTAs of a cluster split the contraction.  Bound by
+// reading X.
+// The tensor cores cut off, rather than round, what a sum's exponent leaves no
+// room for, so the error of a chain of accumulations grows with its length
+// (1.2e-6 of T after 1024 elements, 3.5e-7 after 256).  T is FP32, so the
+// stages go to up to four accumulators in turn, which are added in FP32 at
+// the end.
 template <bool MNB>
 __global__ void __launch_bounds__(kThreads)
     k_low_rank(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapA,
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(kThreads)
   const int kb0 = (int)((int64_t)g.nkb * rank / splits);
   const int kb1 = (int)((int64_t)g.nkb * (rank + 1) / splits);
   uint32_t cols = 32;
-  while (cols < (uint32_t)g.rp) cols *= 2;
+  while (cols < (uint32_t)(g.rp * g.nacc)) cols *= 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < g.xstages; ++i) {
@@ -409,6 +422,8 @@ __global__ void __launch_bounds__(kThreads)
         ok = mbar_wait(&xfull[rx.s], rx.ph, s_abort, g.status, g.budget_ns);
         if (!ok) break;
         const uint32_t x0 = smem_u32(sX + rx.s * x_bytes);
+        const uint32_t d = tmem + (uint32_t)((kb - kb0) % g.nacc * g.rp);
+        const bool more = kb - kb0 >= g.nacc;
         for (int j = 0; j < n; ++j) {
           ok = mbar_wait(&afull[ra.s], ra.ph, s_abort, g.status, g.budget_ns);
           if (!ok) break;
@@ -416,10 +431,10 @@ __global__ void __launch_bounds__(kThreads)
           const uint32_t a0 = smem_u32(sA + ra.s * a_bytes);
 #pragma unroll
           for (int kk = 0; kk < kKB / 16; ++kk)
-            umma_16_masked(tmem, umma_desc_sw128(x0 + kk * 32),
+            umma_16_masked(d, umma_desc_sw128(x0 + kk * 32),
                            MNB ? umma_desc_mn128(a0 + kk * 2048, 8192)
                                : umma_desc_sw128(a0 + kk * 32),
-                           idesc, (kb != kb0) || kk != 0, slots.off[j][0], slots.off[j][1],
+                           idesc, more || kk != 0, slots.off[j][0], slots.off[j][1],
                            slots.off[j][2], slots.off[j][3]);
           umma_commit(&aempty[ra.s]);
           ra.next();
@@ -445,12 +460,19 @@ __global__ void __launch_bounds__(kThreads)
     const int r = q * 32 + lane;
     if (q * 32 < mrows)
       for (int c = 0; c < g.rp; c += 16) {
-        uint32_t v[16];
-        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
-        tmem_wait_ld();
+        float sum[16];
+        const int used = kb1 - kb0 < g.nacc ? kb1 - kb0 : g.nacc;
+        for (int a = 0; a < used; ++a) {
+          uint32_t v[16];
+          tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + a * g.rp + c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            sum[i] = a ? sum[i] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
+        }
         if (r < mrows)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[r * ldp + c + i] = __uint_as_float(v[i]);
+          for (int i = 0; i < 16; ++i) part[r * ldp + c + i] = sum[i];
       }
   }
   cluster_sync();
@@ -574,13 +596,11 @@ int launch_pad_rows(const void* src, int64_t lds, void* dst, int64_t ldd, int64_
 
 namespace {
 
-template <typename... Params, typename... Args>
-int launch_cluster(const char* what, void (*kern)(Params...), int64_t tiles, int splits,
-                   int threads, size_t smem, bool early, cudaStream_t stream, Args... args) {
-  static_assert(sizeof...(Params) == sizeof...(Args), "");
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)smem);
-  if (e != cudaSuccess) return set_cuda_error(what, e);
+template <auto K, typename... Args>
+int launch_cluster(const char* what, int64_t tiles, int splits, int threads, size_t smem,
+                   bool early, int dev, cudaStream_t stream, const Args&... args) {
+  int rc = allow_smem<K>(smem, dev);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * splits));
   cfg.blockDim = dim3(threads);
@@ -595,7 +615,7 @@ int launch_cluster(const char* what, void (*kern)(Params...), int64_t tiles, int
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = early ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, args...);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, K, args...);
   return e == cudaSuccess ? OZK_OK : set_cuda_error(what, e);
 }
 
@@ -642,6 +662,9 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= 2 * device_sm_count(dev) && g.nkb >= splits * 4)
     splits *= 2;
+  // Chains of at most 512 elements where eight CTAs and the accumulators allow it.
+  g.nacc = g.rp <= 64 ? 4 : 2;
+  while (splits < 8 && g.nkb > 8 * splits * g.nacc) splits *= 2;
   const int a_bytes = p.back ? (g.rp + 63) / 64 * 8192 : g.rp * 128;
   g.xstages = 4;
   g.astages = 4;
@@ -651,7 +674,7 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   const size_t red = (size_t)kRows * (g.rp + 1) * 4;
   if (area < need) area = need;
   if (area < red) area = red;
-  if (area < tmem_share(g.rp)) area = tmem_share(g.rp);
+  if (area < tmem_share(g.rp * g.nacc)) area = tmem_share(g.rp * g.nacc);
   CUtensorMap mx, ma;
   int rc;
   if ((rc = make_map(&mx, p.X.p, 2, p.n_in, p.M, 1, p.X.ld * 2, p.X.ld * 2 * p.M, kKB, g.xrows,
@@ -662,10 +685,10 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   else
     rc = make_map(&ma, p.A.p, 2, p.n_in, p.r, p.E, p.A.ld * 2, p.A.ld * 2 * p.r, kKB, g.rp, true);
   if (rc) return rc;
-  return p.back ? launch_cluster("k_low_rank", k_low_rank<true>, tiles, splits, kThreads,
-                                 area + 1024, false, stream, mx, ma, g)
-                : launch_cluster("k_low_rank", k_low_rank<false>, tiles, splits, kThreads,
-                                 area + 1024, false, stream, mx, ma, g);
+  return p.back ? launch_cluster<k_low_rank<true>>("k_low_rank", tiles, splits, kThreads,
+                                                   area + 1024, false, dev, stream, mx, ma, g)
+                : launch_cluster<k_low_rank<false>>("k_low_rank", tiles, splits, kThreads,
+                                                    area + 1024, false, dev, stream, mx, ma, g);
 }
 
 template <int BN, bool MNB>
@@ -702,8 +725,8 @@ int run_linear_bn(const Product& p, LinearArgs g, const uint16_t* split, int spl
                     true);
   }
   if (rc) return rc;
-  return launch_cluster("k_linear", k_linear<BN, MNB>, tiles, splits, kThreads, area + 1024, true,
-                        stream, mx, mw, mt, mb, g);
+  return launch_cluster<k_linear<BN, MNB>>("k_linear", tiles, splits, kThreads, area + 1024, true,
+                                           dev, stream, mx, mw, mt, mb, g);
 }
 
 int run_linear(const Product& p, const int32_t* ids, const uint16_t* split, void* Y, int64_t ldy,
@@ -797,11 +820,13 @@ static int adapter_args(const void* X, int64_t ldx, const void* W, int64_t ldw, 
 
 extern "C" {
 
-size_t ozk_matmul_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E) {
+size_t ozk_matmul_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E,
+                                           int aligned) {
   if (M < 1 || N < 1 || K < 1 || r < 1 || r > kMaxRank || E < 1) return 0;
   Arena ws(nullptr);
   ws.take<uint16_t>((size_t)M * 4 * split_half(r));
-  // The worst case: every operand has to be copied to be aligned.
+  if (aligned) return ws.used;
+  // The worst case: every operand has to be copied.
   ws.take((size_t)M * round_up(K, 8) * 2);
   ws.take((size_t)N * round_up(K, 8) * 2);
   ws.take((size_t)E * r * round_up(K, 8) * 2);
@@ -840,7 +865,8 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
   return run_linear(p, ids, split, Y, ldy, status_dev, dev, s);
 }
 
-size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E) {
+size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E,
+                                         int aligned) {
   if (M < 1 || N < 1 || K < 1 || r < 1 || r > kMaxRank || E < 1) return 0;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -848,6 +874,7 @@ size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r,
   ws.take((size_t)M * 4 * split_half(r));
   ws.take((size_t)M * r * 4);
   ws.take(outer_scratch_bytes(M, N, K, r, E, dev));
+  if (aligned) return ws.used;
   ws.take((size_t)M * round_up(N, 8) * 2);
   ws.take((size_t)N * round_up(K, 8) * 2);
   ws.take((size_t)E * r * round_up(K, 8) * 2);

@@ -366,9 +366,12 @@ __global__ void k_outer_join(const __grid_constant__ OuterArgs g) {
   }
 }
 
-// Rows per chunk: enough chunks for two CTAs per SM, each of at least 256 rows.
+// Rows per chunk: the most chunks that run at once, two CTAs per SM, each of at
+// least 256 rows (a second wave of a few CTAs would double the time).
 int chunk_len(int64_t M, int64_t tiles, int sms) {
-  int64_t len = round_up(M * tiles / (2 * sms) + 1, kStep);
+  int64_t chunks = 2 * sms / tiles;
+  if (chunks < 1) chunks = 1;
+  int64_t len = round_up((M + chunks - 1) / chunks, kStep);
   if (len < 256) len = 256;
   if (len > 8192) len = 8192;
   return (int)len;
@@ -432,8 +435,8 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
   size_t smem = 1024 + 2 * (size_t)(kZBytes + 2 * ((g.rp + 63) / 64) * 8192);
   if (smem < tmem_share(2 * g.rp)) smem = tmem_share(2 * g.rp);
   auto kern = p.bf16 ? k_outer<true> : k_outer<false>;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(k_outer)", e);
+  int rc = p.bf16 ? allow_smem<k_outer<true>>(smem, dev) : allow_smem<k_outer<false>>(smem, dev);
+  if (rc) return rc;
   kern<<<dim3((unsigned)tiles, (unsigned)chunks), kOuterThreads, smem, stream>>>(g);
   e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error("k_outer launch", e);

@@ -8,6 +8,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <mutex>
+
 #include "ozaki_b200.h"
 #include "ozk_internal.h"
 
@@ -783,5 +785,28 @@ int ozk_set_l2_persisting(size_t bytes, size_t* previous) {
 }
 
 const char* ozk_version(void) { return "ozaki-b200 0.1.0 (sm_100a)"; }
+
+int ozk_status_word(int32_t** word) {
+  if (!word) return set_error(OZK_ERR_ARG, "NULL word");
+  static std::mutex m;
+  static int32_t* words[64] = {nullptr};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64) return set_cuda_error("cudaGetDevice", e);
+  std::lock_guard<std::mutex> lock(m);
+  if (!words[dev]) {
+    // Pinned memory may be asked for while another stream is being captured.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    int32_t* p = nullptr;
+    e = cudaHostAlloc((void**)&p, sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return set_cuda_error("cudaHostAlloc", e);
+    *p = 0;
+    words[dev] = p;
+  }
+  *word = words[dev];
+  return OZK_OK;
+}
 
 }  // extern "C"

@@ -266,12 +266,12 @@ int ozk_restore_rows(const void* codes, int64_t ldc, const void* exps, int64_t M
   return e == cudaSuccess ? OZK_OK : set_cuda_error("k_restore_rows launch", e);
 }
 
-size_t ozk_checkpoint_grad_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+size_t ozk_checkpoint_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int aligned) {
   if (M < 1 || N < 1 || K < 1) return 0;
   int dev = 0;
   cudaGetDevice(&dev);
   Arena ws(nullptr);
-  ws.take((size_t)M * round_up(N, 8) * 2);  // dY, if it has to be copied to be aligned
+  if (!aligned) ws.take((size_t)M * round_up(N, 8) * 2);  // room for dY's copy
   ws.take(wide_partial_bytes(N, K, M, dev));
   return ws.used;
 }

@@ -7,6 +7,8 @@
 #include "ozk_device.cuh"
 #include "ozk_internal.h"
 
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -273,6 +275,19 @@ inline size_t tmem_share(int cols) {
   int c = 32;
   while (c < cols) c *= 2;
   return (size_t)c * 456;
+}
+
+// Lets kernel K use `bytes` of dynamic shared memory on device dev; the driver
+// is asked once per size that is larger than those before.
+template <auto K>
+int allow_smem(size_t bytes, int dev) {
+  static std::atomic<int> allowed[64];
+  if (dev < 0 || dev >= 64) return set_error(OZK_ERR_ARG, "device %d", dev);
+  if ((int)bytes <= allowed[dev].load(std::memory_order_relaxed)) return OZK_OK;
+  cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute", e);
+  allowed[dev].store((int)bytes, std::memory_order_relaxed);
+  return OZK_OK;
 }
 
 // Carves aligned areas out of a caller's workspace (or, with base NULL, only counts them).

@@ -54,6 +54,7 @@ struct WideCfg {
 struct WideArgs {
   int64_t M, N;
   int nkb, tiles_m, tiles_n, group_m, splits;
+  int chain;           // stages summed in one accumulator before FP32 takes over
   int bf16, out_f32, accumulate, o_vec;
   void* out;
   int64_t ldo;
@@ -77,57 +78,55 @@ __device__ __forceinline__ void tile_at(const WideArgs& g, int t, int& tm, int& 
   tn = r / rows;
 }
 
-// 32 consecutive outputs of one row, n of them inside the matrix.
-__device__ __forceinline__ void store_row(const WideArgs& g, int64_t row, int64_t col, int n,
-                                          const uint32_t (&v)[32]) {
-  if (g.out_f32) {
-    float* o = (float*)g.out + row * g.ldo + col;
-    if (g.o_vec && n >= 32) {
+// 32 consecutive outputs of one row, n of them inside the matrix, added to
+// what is there with `add`.
+__device__ __forceinline__ void store_f32(float* o, bool vec, int n, const uint32_t (&v)[32],
+                                          bool add) {
+  if (vec && n >= 32) {
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        float4 q = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]),
-                               __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-        if (g.accumulate) {
-          const float4 p = *(const float4*)(o + i);
-          q.x += p.x, q.y += p.y, q.z += p.z, q.w += p.w;
-        }
-        *(float4*)(o + i) = q;
+    for (int i = 0; i < 32; i += 4) {
+      float4 q = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]),
+                             __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+      if (add) {
+        const float4 p = *(const float4*)(o + i);
+        q.x += p.x, q.y += p.y, q.z += p.z, q.w += p.w;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < n) o[i] = __uint_as_float(v[i]) + (g.accumulate ? o[i] : 0.0f);
+      *(float4*)(o + i) = q;
     }
   } else {
-    uint16_t* o = (uint16_t*)g.out + row * g.ldo + col;
-    if (g.o_vec && n >= 32) {
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        float f[8];
+    for (int i = 0; i < 32; ++i)
+      if (i < n) o[i] = __uint_as_float(v[i]) + (add ? o[i] : 0.0f);
+  }
+}
+__device__ __forceinline__ void store_16(uint16_t* o, bool vec, int n, const uint32_t (&v)[32],
+                                         bool add, bool bf16) {
+  if (vec && n >= 32) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[i + j]);
-        if (g.accumulate) {
-          const uint4 p = *(const uint4*)(o + i);
-          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+    for (int i = 0; i < 32; i += 8) {
+      float f[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            f[2 * j] += widen16(g.bf16, (uint16_t)w[j]);
-            f[2 * j + 1] += widen16(g.bf16, (uint16_t)(w[j] >> 16));
-          }
+      for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[i + j]);
+      if (add) {
+        const uint4 p = *(const uint4*)(o + i);
+        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[2 * j] += widen16(bf16, (uint16_t)w[j]);
+          f[2 * j + 1] += widen16(bf16, (uint16_t)(w[j] >> 16));
         }
-        uint4 q;
-        q.x = pack16(g.bf16, f[0], f[1]);
-        q.y = pack16(g.bf16, f[2], f[3]);
-        q.z = pack16(g.bf16, f[4], f[5]);
-        q.w = pack16(g.bf16, f[6], f[7]);
-        *(uint4*)(o + i) = q;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < n)
-          o[i] = round16(g.bf16, __uint_as_float(v[i]) + (g.accumulate ? widen16(g.bf16, o[i]) : 0.0f));
+      uint4 q;
+      q.x = pack16(bf16, f[0], f[1]);
+      q.y = pack16(bf16, f[2], f[3]);
+      q.z = pack16(bf16, f[4], f[5]);
+      q.w = pack16(bf16, f[6], f[7]);
+      *(uint4*)(o + i) = q;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) o[i] = round16(bf16, __uint_as_float(v[i]) + (add ? widen16(bf16, o[i]) : 0.0f));
   }
 }
 
@@ -260,19 +259,29 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
       for (int i = unit; ok && i < items; i += n_units, ++it) {
         int tm, tn, sp, kb0, kb1;
         item_at(i, tm, tn, sp, kb0, kb1);
-        const int buf = it & 1;
-        ok = mbar_wait(&acce[buf], ((it >> 1) & 1) ^ 1, s_abort, g.status, g.budget_ns);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t d = tmem + buf * kTile;
+        int buf = it & 1;
+        uint32_t d = tmem + buf * kTile;
+        int head = kb0;  // first stage of this accumulator's chain
         for (int kb = kb0; kb < kb1; ++kb) {
+          if (kb == kb0 || kb - head == g.chain) {
+            if (kb != kb0) {
+              umma_commit_pair(&accf[buf], 0x3);
+              ++it;
+            }
+            buf = it & 1;
+            d = tmem + buf * kTile;
+            head = kb;
+            ok = mbar_wait(&acce[buf], ((it >> 1) & 1) ^ 1, s_abort, g.status, g.budget_ns);
+            if (!ok) break;
+            tc_fence_after();
+          }
           ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
           if (!ok) break;
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + rg.s * kStageBytes), b0 = a0 + kABytes;
 #pragma unroll
           for (int kk = 0; kk < kKB / 16; ++kk)
-            umma_bf16_pair(d, desc_a(a0, kk), desc_b(b0, kk), idesc, kb != kb0 || kk != 0);
+            umma_bf16_pair(d, desc_a(a0, kk), desc_b(b0, kk), idesc, kb != head || kk != 0);
           umma_commit_pair(&empty[rg.s], 0x3);
           rg.next();
         }
@@ -316,11 +325,15 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;
     int it = 0;
-    for (int i = unit; i < items; i += n_units, ++it) {
+    bool ok = true;
+    for (int i = unit; ok && i < items; i += n_units) {
       int tm, tn, sp, kb0, kb1;
       item_at(i, tm, tn, sp, kb0, kb1);
+      for (int head = kb0; head < kb1; head += g.chain, ++it) {
       const int buf = it & 1;
-      if (!mbar_wait(&accf[buf], (it >> 1) & 1, s_abort, g.status, g.budget_ns)) break;
+      ok = mbar_wait(&accf[buf], (it >> 1) & 1, s_abort, g.status, g.budget_ns);
+      if (!ok) break;
+      const bool add = head != kb0;  // this thread wrote the sum so far
       tc_fence_after();
       const int64_t row = (int64_t)tm * kTile + rank * kHalf + q * 32 + lane;
       const int64_t col0 = (int64_t)tn * kTile;
@@ -340,20 +353,14 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
         if (row >= g.M || left <= 0) continue;
         const int n = left < 32 ? (int)left : 32;
         if (g.splits > 1) {
-          float* o = g.partial + ((int64_t)sp * g.M + row) * g.N + col0 + c;
-          if (n == 32 && (g.N & 3) == 0) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *(float4*)(o + j) = make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]),
-                                              __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < n) o[j] = __uint_as_float(v[j]);
-          }
+          store_f32(g.partial + ((int64_t)sp * g.M + row) * g.N + col0 + c, (g.N & 3) == 0, n, v,
+                    add);
+        } else if (g.out_f32) {
+          store_f32((float*)g.out + row * g.ldo + col0 + c, g.o_vec, n, v, add || g.accumulate);
         } else {
-          store_row(g, row, col0 + c, n, v);
+          store_16((uint16_t*)g.out + row * g.ldo + col0 + c, g.o_vec, n, v, g.accumulate, BF16);
         }
+      }
       }
     }
   } else if constexpr (MODE == kWideWeight) {
@@ -529,8 +536,9 @@ int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) 
     if (rc) return rc;
   }
   auto kern = p.bf16 ? k_wide<MODE, true> : k_wide<MODE, false>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
-  if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(k_wide)", e);
+  if ((rc = p.bf16 ? allow_smem<k_wide<MODE, true>>(Cfg::SMEM, dev)
+                   : allow_smem<k_wide<MODE, false>>(Cfg::SMEM, dev)))
+    return rc;
   const int items = g.tiles_m * g.tiles_n * g.splits;
   const int units = device_sm_count(dev) / 2;
   cudaLaunchConfig_t cfg = {};
@@ -547,7 +555,7 @@ int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.early ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, ma, mb, mt, mbi, g);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ma, mb, mt, mbi, g);
   return e == cudaSuccess ? OZK_OK : set_cuda_error("k_wide launch", e);
 }
 
@@ -570,6 +578,11 @@ int launch_wide(const WideProduct& p, int dev, cudaStream_t stream) {
   g.tiles_n = (int)tn;
   g.group_m = 8;
   g.splits = p.mode == kWideWeight && p.partial ? wide_splits(p.M, p.N, p.C, dev) : 1;
+  // The tensor cores cut off what a sum's exponent leaves no room for, so an
+  // error grows with the length of the chain: an FP32 result was 1.7e-5 off
+  // after 16384 FP16 rows, 7e-7 after 1024.  FP32 results are summed in chains
+  // of 1024; a 16-bit rounding hides it.
+  g.chain = p.out_f32 || g.splits > 1 ? 16 : 1 << 30;
   g.bf16 = p.bf16;
   g.out_f32 = p.out_f32;
   g.accumulate = p.accumulate;

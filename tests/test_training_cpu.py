@@ -119,8 +119,9 @@ def test_entry_points_refuse_before_device_work():
     assert forward(M=1 << 31) == UNS
     assert forward() == WS and forward(ws=p, n=16) == WS
     assert forward(M=0) == OK and forward(N=0) == OK
-    assert lib.ozk_matmul_adapters_workspace_bytes(4, 8, 16, 4, 2) > 0
-    assert lib.ozk_matmul_adapters_workspace_bytes(0, 8, 16, 4, 2) == 0
+    assert lib.ozk_matmul_adapters_workspace_bytes(4, 8, 16, 4, 2, 0) > \
+        lib.ozk_matmul_adapters_workspace_bytes(4, 8, 16, 4, 2, 1) > 0
+    assert lib.ozk_matmul_adapters_workspace_bytes(0, 8, 16, 4, 2, 1) == 0
 
     def grad(dY=p, ldy=8, X=p, ldx=16, exps=None, W=p, ldw=16, T=p, dX=p, lddx=16, dA=p, dB=p, M=4,
              N=8, K=16, r=4, E=2, dt=0, ws=None, n=0):
@@ -153,4 +154,5 @@ def test_entry_points_refuse_before_device_work():
     assert wg(p, 8, p, 128, p, p, 4, 2, 8, 4, 0, 1, 0, None, 0, None, None) == ARG
     assert wg(p, 9, p, 128, p, p, 4, 2, 9, 4, 0, 0, 0, None, 0, None, None) == WS
     assert wg(p, 8, p, 128, p, p, 4, 2, 0, 4, 0, 0, 0, None, 0, None, None) == OK
+    assert lib.ozk_status_word(None) == ARG
     assert _lib.detail()
