@@ -314,16 +314,6 @@ struct LowArgs {
   uint64_t budget_ns;
 };
 
-// Rounds t to its high and low 16-bit parts and stores them in the split T.
-__device__ __forceinline__ void store_split(uint16_t* split, int64_t row, int half, int c, float t,
-                                            bool bf16) {
-  const uint16_t hi = round16(bf16, t);
-  float rest = t - widen16(bf16, hi);
-  if (!(fabsf(rest) <= 3.0e38f)) rest = 0.0f;  // t not finite: hi says so by itself
-  split[row * 2 * half + c] = hi;
-  split[row * 2 * half + half + c] = round16(bf16, rest);
-}
-
 // T of a tile of 128 rows: each block of 64 contraction elements of X is loaded
 // once and multiplied with the same block of every adapter of the tile, each
 // into its own lanes.  The CTAs of a cluster split the contraction.  Bound by
@@ -872,7 +862,6 @@ size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r,
   cudaGetDevice(&dev);
   Arena ws(nullptr);
   ws.take((size_t)M * 4 * split_half(r));
-  ws.take((size_t)M * r * 4);
   ws.take(outer_scratch_bytes(M, N, K, r, E, dev));
   if (aligned) return ws.used;
   ws.take((size_t)M * round_up(N, 8) * 2);
@@ -910,7 +899,6 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   Product p = {{dY, ldy}, {W, ldw}, {B, r}, {A, K}, M, K, N, r, E, true, dt == OZK_DT_BF16};
   Arena ws(workspace);
   uint16_t* split = ws.take<uint16_t>((size_t)M * 4 * split_half(r));
-  float* U = ws.take<float>((size_t)M * r * 4);
   void* scratch = ws.take(outer_scratch_bytes(M, N, K, r, E, dev));
   for (int pass = 0; pass < 2; ++pass) {
     Product q = p;
@@ -923,7 +911,7 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
     else if (!workspace || w.used > ws_bytes || ((uintptr_t)workspace & 127))
       return set_error(OZK_ERR_WORKSPACE, "workspace of %zu bytes, aligned to 128, needed", w.used);
   }
-  if ((rc = run_low_rank(p, ids, scale, (float)alpha, U, split, status_dev, dev, s))) return rc;
+  if ((rc = run_low_rank(p, ids, scale, (float)alpha, nullptr, split, status_dev, dev, s))) return rc;
   if (dX && (rc = run_linear(p, ids, split, dX, lddx, status_dev, dev, s))) return rc;
   OuterProduct o = {};
   o.bf16 = p.bf16;
@@ -938,7 +926,7 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   o.exps = (const int8_t*)exps;
   o.dY = p.X.p;
   o.ldy = p.X.ld;
-  o.U = U;
+  o.U = split;
   o.T = T;
   o.dA = dA;
   o.dB = dB;

@@ -16,7 +16,8 @@ struct OuterProduct {
   const int8_t* exps;
   const void* dY;       // [M][N]
   int64_t ldy;
-  const float *U, *T;   // [M][r]
+  const uint16_t* U;    // [M][2 split_half(r)]: high and low parts
+  const float* T;       // [M][r]
   void *dA, *dB;        // [E][r][K], [E][N][r]
   int32_t* status;
 };

@@ -7,10 +7,15 @@
 // reading X and dY once.
 //
 // k_sort_rows lists the rows by adapter (stable, one CTA per adapter, no
-// atomics).  k_outer cuts that list into chunks; a CTA takes one chunk and 256
-// columns, gathers 64 rows at a time into shared memory (converting codes, and
-// splitting U or T into high and low 16-bit parts, on the way) and multiplies
-// them on the tensor cores: D[256 columns][r] += Z^T [hi | lo].  Rows of other
+// atomics on memory) and splits T into high and low 16-bit parts, as U already
+// is.  k_outer cuts the list into chunks; a CTA takes one chunk and 256 columns,
+// gathers 64 rows at a time into a ring of shared-memory stages (cp.async, three
+// stages in flight: 96 KB per SM; codes are converted on the way to the tensor
+// cores) and multiplies them: D[256 columns][2 r] += Z^T [hi | lo], the halves
+// being added at the end.  One warp issues the MMAs (about 90 clocks each at
+// these widths, bound by reading Z from shared memory) and one looks the next
+// rows up, beside the sixteen that fetch: with the issue and the lookup in the
+// fetching warps a stage took 5400 clocks.  Rows of other
 // adapters are never read, so a NaN in them cannot reach this one's gradient.
 // A chunk that holds all of an adapter's rows writes its gradient at once;
 // otherwise the chunks' FP32 sums are added in order by k_outer_join: the
@@ -28,15 +33,30 @@ namespace ozk {
 namespace {
 
 constexpr int kSortThreads = 1024;
-constexpr int kOuterThreads = 256;
+constexpr int kOuterWarps = 16;  // that fetch and convert; two more issue MMAs and look rows up
+constexpr int kOuterFetch = 32 * kOuterWarps;
+constexpr int kOuterThreads = kOuterFetch + 64;
 constexpr int kCols = 256;       // columns of Z per CTA: two accumulators of 128
 constexpr int kStep = 64;        // rows per stage
 constexpr int kZBytes = kCols * kStep * 2;
+constexpr int kZRows = kStep / kOuterWarps;  // rows of a stage that a warp fetches
 
 // order: the rows of adapters 0, 1, ... in turn, each adapter's in ascending
 // order; start[e]: the first place of adapter e.
 __global__ void __launch_bounds__(kSortThreads)
-    k_sort_rows(const int32_t* ids, int64_t M, int E, int32_t* order, int32_t* start) {
+    k_sort_rows(const int32_t* ids, int64_t M, int E, int32_t* order, int32_t* start,
+                const float* T, int r, uint16_t* split, int bf16) {
+  if ((int)blockIdx.x >= E) {  // the CTAs after the adapters': the split of T
+    const int half = split_half(r);
+    const int64_t n = M * half;
+    for (int64_t i = (int64_t)((int)blockIdx.x - E) * kSortThreads + threadIdx.x; i < n;
+         i += (int64_t)((int)gridDim.x - E) * kSortThreads) {
+      const int64_t m = i / half;
+      const int c = (int)(i - m * half);
+      store_split(split, m, half, c, c < r ? T[m * r + c] : 0.0f, bf16);
+    }
+    return;
+  }
   __shared__ int s_less, s_eq;
   __shared__ int s_warp[kSortThreads / 32];
   const int e = blockIdx.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -84,7 +104,7 @@ struct OuterJob {
   const void* Z;         // 16-bit [M][C], or int8 codes when exps is set
   int64_t ldz, C;
   const int8_t* exps;    // [groups][M]
-  const float* L;        // [M][r]
+  const uint16_t* L;     // [M][2 split_half(r)]: high parts, low parts
   float* partial;        // [chunks + E][r C]
   void* out;             // [E][r][C], or [E][C][r] when trans
   int trans, tiles, vec;
@@ -125,228 +145,281 @@ struct Walk {
   }
 };
 
-template <bool BF16>
-__global__ void __launch_bounds__(kOuterThreads, 2)
-    k_outer(const __grid_constant__ OuterArgs g) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t empty[2], done;
-  __shared__ uint32_t s_tmem;
-  __shared__ int s_rows[2][kStep];
-  __shared__ int s_abort_word;
-  volatile int* s_abort = &s_abort_word;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+constexpr int kRowSlots = 8;  // stages whose row numbers are held
+
+struct OuterShared {
+  uint64_t empty[4], done;
+  uint32_t tmem;
+  int abort;
+  int rows[kRowSlots][kStep];
+};
+
+// One chunk and 256 columns.  A stage holds Z (32 KB, or 16 KB of codes) and
+// L's rows, high parts then low parts; with CODES two buffers of 32 KB behind the ring take
+// the converted Z in turn.
+template <bool BF16, bool CODES, int S>
+__device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0, int chunk,
+                           int limit, uint8_t* smem, OuterShared& sh) {
+  constexpr int Z_STAGE = CODES ? kZBytes / 2 : kZBytes;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const bool second = (int)blockIdx.x >= g.job[0].tiles;
-  const OuterJob& job = g.job[second];
-  const int64_t col0 = (int64_t)((int)blockIdx.x - (second ? g.job[0].tiles : 0)) * kCols;
-  const int chunk = blockIdx.y;
-  const int total = __ldg(g.start + g.E);
-  const int c0 = chunk * g.len;
-  const int limit = c0 + g.len < total ? c0 + g.len : total;
-  if (c0 >= limit) return;  // the whole CTA: nothing is allocated yet
-  const int lblk = (g.rp + 63) / 64;  // 8 KB blocks of a part of L
-  const int stage_bytes = kZBytes + 2 * lblk * 8192;
-  uint32_t cols = 32;
-  while (cols < 2u * g.rp) cols *= 2;
+  const int stage_bytes = Z_STAGE + (2 * g.rp + 63) / 64 * 8192;
+  uint8_t* conv = smem + S * stage_bytes;
+  const uint32_t tmem = sh.tmem;
+  volatile int* s_abort = &sh.abort;
+  const int half = split_half(g.r);
+  const bool fetcher = warp < kOuterWarps;
 
-  if (t == 0) {
-    mbar_init(&empty[0], 1);
-    mbar_init(&empty[1], 1);
-    mbar_init(&done, 1);
-    *s_abort = 0;
-    fence_mbar_init();
-  }
-  if (warp == 0) tmem_alloc(&s_tmem, cols);
-
-  // The first adapter of the chunk: the last e with start[e] <= c0 and rows there.
-  Walk cur, nxt;
+  // The first adapter of the chunk: the last e with start[e] <= its first place.
+  Walk cur;
+  cur.pos = chunk * g.len;
   {
-    int lo = 0, hi = g.E - 1;  // start[lo] <= c0
+    int lo = 0, hi = g.E - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (__ldg(g.start + mid) <= c0) lo = mid;
+      if (__ldg(g.start + mid) <= cur.pos) lo = mid;
       else hi = mid - 1;
     }
     cur.e = lo;
-    cur.pos = c0;
     cur.seek(g.start, g.E, limit);
   }
-  nxt = cur;
-  nxt.next(g.start, g.E, limit);
-  auto rows_of = [&](const Walk& w, int slot) {
-    if (t < kStep) s_rows[slot][t] = w.e < g.E && w.pos + t < w.end ? __ldg(g.order + w.pos + t) : -1;
+  // cur: the stage being multiplied; ahead: the one whose row numbers come next.
+  Walk ahead = cur;
+  auto number_rows = [&](int stage) {
+#pragma unroll
+    for (int i = 0; i < kStep; i += 32) {
+      const int p = ahead.pos + i + lane;
+      sh.rows[stage % kRowSlots][i + lane] = ahead.e < g.E && p < ahead.end ? __ldg(g.order + p) : -1;
+    }
+    ahead.next(g.start, g.E, limit);
   };
-  rows_of(cur, 0);
-  rows_of(nxt, 1);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = s_tmem;
-
-  // A stage in registers: Z rows warp + 8 j, 8 columns at 8 lane; L pieces of 8
-  // ranks, piece t + 256 i being row (t + 256 i) / (rp / 8).
-  uint4 z[8];
-  uint32_t sc[8];
-  float l[4][8];
-  const int lp = g.rp / 8;
   const int64_t col = col0 + lane * 8;
-  auto fetch = [&](int slot) {
+  const uint32_t swz = (uint32_t)(lane & 7) << 4;  // this lane's piece of a 128-byte line
+  // This thread's 16-byte pieces of L's parts: the row, where it comes from in
+  // that row, where it goes in a stage.
+  const int lp = g.rp / 8, pieces = 2 * kStep * lp;
+  int l_row[4], l_from[4];
+  uint32_t l_to[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int row = s_rows[slot][warp + 8 * j];
-      z[j] = make_uint4(0, 0, 0, 0);
-      sc[j] = 0;
-      if (row < 0) continue;
-      if (job.exps) {
-        const int64_t ldc = job.ldz;
-        if (col < ldc) {
-          const uint2 q = __ldg((const uint2*)((const int8_t*)job.Z + (int64_t)row * ldc + col));
-          z[j].x = q.x;
-          z[j].y = q.y;
-          sc[j] = (uint32_t)(int)__ldg(job.exps + (col / kGroup) * g.M + row);
-        }
+  for (int i = 0; i < 4; ++i) {
+    const int q = t + i * kOuterFetch;
+    const int r = q / (2 * lp), c = q - r * 2 * lp;  // piece c of the row's 2 lp
+    const int part = c >= lp;
+    l_row[i] = q < pieces ? r : -1;
+    l_from[i] = 2 * (part * half + (c - part * lp) * 8);
+    l_to[i] = Z_STAGE + (c >> 3) * 8192 + r * 128 + (((uint32_t)(c & 7) ^ (uint32_t)(r & 7)) << 4);
+  }
+  // What does not change from stage to stage: this lane's bytes of a row of Z
+  // (its 8 columns, or those of them inside the matrix) and where they go.
+  const int64_t left = (CODES ? job.ldz : job.C) - col;
+  const uint32_t z_bytes = left <= 0 ? 0 : CODES ? 8 : left < 8 ? 2 * (uint32_t)left : 16;
+  const int64_t z_pitch = job.ldz * (CODES ? 1 : 2);
+  const char* z_from = (const char*)job.Z + (z_bytes ? col * (CODES ? 1 : 2) : 0);
+  const bool vec = CODES || job.vec;
+  uint32_t z_to[kZRows];
+#pragma unroll
+  for (int j = 0; j < kZRows; ++j) {
+    const int r = warp + kOuterWarps * j;
+    z_to[j] = CODES ? r * 256 + lane * 8
+                    : (lane >> 3) * 8192 + r * 128 + (swz ^ ((uint32_t)(r & 7) << 4));
+  }
+  const char* l_base = (const char*)job.L;
+  const int l_pitch = 4 * half;
+  auto load = [&](uint32_t zb, const int* rows) {
+#pragma unroll
+    for (int j = 0; j < kZRows; ++j) {
+      const int row = rows[warp + kOuterWarps * j];
+      const char* p = z_from + (row >= 0 ? row : 0) * z_pitch;
+      const uint32_t n = row >= 0 ? z_bytes : 0;
+      if constexpr (CODES) {
+        cp_async8(zb + z_to[j], p, n);
+      } else if (vec) {
+        cp_async16(zb + z_to[j], p, n);
       } else {
-        const uint16_t* p = (const uint16_t*)job.Z + (int64_t)row * job.ldz + col;
-        if (job.vec && col + 8 <= job.C) {
-          z[j] = __ldg((const uint4*)p);
-        } else {
-          uint32_t w[4];
+        const uint16_t* e = (const uint16_t*)p;
+        uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t a = col + 2 * i < job.C ? p[2 * i] : 0;
-            const uint32_t b = col + 2 * i + 1 < job.C ? p[2 * i + 1] : 0;
-            w[i] = a | (b << 16);
-          }
-          z[j] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int i = 0; i < 4; ++i)
+          w[i] = (4 * i < n ? e[2 * i] : 0u) | ((4 * i + 2 < n ? e[2 * i + 1] : 0u) << 16);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(zb + z_to[j]), "r"(w[0]),
+                     "r"(w[1]), "r"(w[2]), "r"(w[3])
+                     : "memory");
       }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int q = t + kOuterThreads * i;
-      if (q >= kStep * lp) break;
-      const int row = s_rows[slot][q / lp], c = q % lp * 8;
-      const float* p = job.L + (int64_t)row * g.r + c;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) l[i][k] = row >= 0 && c + k < g.r ? __ldg(p + k) : 0.0f;
+      if (l_row[i] < 0) break;
+      const int row = rows[l_row[i]];
+      cp_async16(zb + l_to[i], l_base + (int64_t)(row >= 0 ? row : 0) * l_pitch + l_from[i],
+                 row >= 0 ? 16 : 0);
     }
   };
-  auto put = [&](uint8_t* st) {
-    const uint32_t zb = smem_u32(st) + (lane >> 3) * 8192;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int row = warp + 8 * j;
-      uint32_t w[4] = {z[j].x, z[j].y, z[j].z, z[j].w};
-      if (job.exps) {
-        const uint32_t s = exp_pair(BF16, (int)sc[j]);
-        codes_to_16(BF16, z[j].y, s, w[2], w[3]);
-        codes_to_16(BF16, z[j].x, s, w[0], w[1]);
-      }
-      const uint32_t at = zb + row * 128 + (((uint32_t)(lane & 7) ^ (uint32_t)(row & 7)) << 4);
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
-                   "r"(w[2]), "r"(w[3])
-                   : "memory");
-    }
-    const uint32_t lb = smem_u32(st) + kZBytes;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int q = t + kOuterThreads * i;
-      if (q >= kStep * lp) break;
-      const int row = q / lp, c8 = q % lp;
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float a = l[i][2 * k], b = l[i][2 * k + 1];
-        hi[k] = pack16(BF16, a, b);
-        float ra = a - widen16(BF16, (uint16_t)hi[k]), rb = b - widen16(BF16, (uint16_t)(hi[k] >> 16));
-        if (!(fabsf(ra) <= 3.0e38f)) ra = 0.0f;
-        if (!(fabsf(rb) <= 3.0e38f)) rb = 0.0f;
-        lo[k] = pack16(BF16, ra, rb);
-      }
-      const uint32_t at = lb + (c8 >> 3) * 8192 + row * 128 +
-                          (((uint32_t)(c8 & 7) ^ (uint32_t)(row & 7)) << 4);
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]),
-                   "r"(hi[2]), "r"(hi[3])
-                   : "memory");
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lblk * 8192), "r"(lo[0]),
-                   "r"(lo[1]), "r"(lo[2]), "r"(lo[3])
-                   : "memory");
-    }
+  // Steps of a stage: lane 4 g + j holds row warp + 16 j of column group g.
+  // (Turned into 16-bit steps when they are used, an iteration later.)
+  auto exponents = [&](int stage) {
+    if (!CODES || !fetcher || lane >= 2 * kZRows) return 0;
+    const int row = sh.rows[stage % kRowSlots][warp + kOuterWarps * (lane % kZRows)];
+    const int64_t group = col0 / kGroup + lane / kZRows;
+    return row >= 0 && group * kGroup < job.ldz ? (int)__ldg(job.exps + group * g.M + row) : 0;
   };
 
-  const uint32_t idesc = umma_idesc_16(BF16, 128, g.rp, true, true);
-  fetch(0);
+  if (warp == kOuterWarps + 1)
+    for (int k = 0; k < S; ++k) number_rows(k);
+  __syncthreads();
+  if (fetcher)
+    for (int k = 0; k < S - 1; ++k) {
+      load(smem_u32(smem) + k * stage_bytes, sh.rows[k]);
+      cp_async_commit();
+    }
+  int ex = exponents(0);
+  const uint32_t idesc = umma_idesc_16(BF16, 128, 2 * g.rp, true, true);
   uint32_t done_ph = 0;
   bool ok = true;
+  int slot = 0, before = S - 1;        // ring places of this stage and of the one before it
+  uint32_t ph = 0, before_ph = 1;      // phase parity of their uses
   for (int it = 0; cur.e < g.E; ++it) {
-    const int buf = it & 1;
-    uint8_t* st = smem + buf * stage_bytes;
-    ok = mbar_wait(&empty[buf], ((it >> 1) & 1) ^ 1, s_abort, g.status, g.budget_ns);
-    if (__syncthreads_or(!ok)) break;  // all threads leave together
-    put(st);
+    uint8_t* st = smem + slot * stage_bytes;
+    cp_async_wait<S - 2>();
+    const uint32_t z0 = CODES ? smem_u32(conv + (it & 1) * kZBytes) : smem_u32(st);
+    if (CODES && fetcher) {
+      const uint32_t steps = exp_pair(BF16, ex);
+      // Every thread converts the pieces that it fetched.  (The multiplication
+      // two stages ago, which read this buffer, has been waited for.)
+#pragma unroll
+      for (int j = 0; j < kZRows; ++j) {
+        const int r = warp + kOuterWarps * j;
+        const uint2 q = *(const uint2*)(st + z_to[j]);
+        const uint32_t step = __shfl_sync(~0u, steps, (lane >> 4) * kZRows + j);
+        uint32_t w[4];
+        codes_to_16(BF16, q.x, step, w[0], w[1]);
+        codes_to_16(BF16, q.y, step, w[2], w[3]);
+        const uint32_t at = z0 + (lane >> 3) * 8192 + r * 128 + (swz ^ ((uint32_t)(r & 7) << 4));
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
+                     "r"(w[2]), "r"(w[3])
+                     : "memory");
+      }
+    }
     fence_proxy_async_smem();
-    __syncthreads();
+    if (__syncthreads_or(!ok)) break;  // all threads leave together
     const bool fresh = cur.pos == cur.first, last = cur.last();
-    if (t == 0) {
+    if (t == kOuterFetch) {
       tc_fence_after();
-      const uint32_t z0 = smem_u32(st), l0 = z0 + kZBytes;
+      const uint32_t l0 = smem_u32(st) + Z_STAGE;
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
+      for (int kk = 0; kk < kStep / 16; ++kk)
 #pragma unroll
-        for (int kk = 0; kk < kStep / 16; ++kk) {
-          const uint64_t da = umma_desc_mn128(z0 + mb * 16384 + kk * 2048, 8192);
-          umma_bf16(tmem + mb * g.rp, da, umma_desc_mn128(l0 + kk * 2048, 8192), idesc,
-                    !fresh || kk != 0);
-          umma_bf16(tmem + mb * g.rp, da, umma_desc_mn128(l0 + lblk * 8192 + kk * 2048, 8192),
-                    idesc, 1);
+        for (int mb = 0; mb < 2; ++mb) {
+          umma_bf16(tmem + mb * 2 * g.rp, umma_desc_mn128(z0 + mb * 16384 + kk * 2048, 8192),
+                    umma_desc_mn128(l0 + kk * 2048, 8192), idesc, !fresh || kk != 0);
         }
-      umma_commit(&empty[buf]);
-      if (last) umma_commit(&done);
+      umma_commit(&sh.empty[slot]);
+      if (last) umma_commit(&sh.done);
+    }
+    // Refill: the stage before this one is free once its multiplication is done.
+    if (fetcher) {
+      if (it > 0) ok = mbar_wait(&sh.empty[before], before_ph, s_abort, g.status, g.budget_ns);
+      if (ok) load(smem_u32(smem) + before * stage_bytes, sh.rows[(it + S - 1) % kRowSlots]);
+      cp_async_commit();
+      ex = exponents(it + 1);
+    } else if (warp == kOuterWarps + 1) {
+      number_rows(it + S);
+    }
+    __syncwarp();
+    before = slot;
+    before_ph = ph;
+    if (++slot == S) {
+      slot = 0;
+      ph ^= 1;
     }
     const Walk was = cur;
-    cur = nxt;
-    nxt.next(g.start, g.E, limit);
-    rows_of(nxt, buf);
-    if (cur.e < g.E) fetch(buf ^ 1);
+    cur.next(g.start, g.E, limit);
     if (last) {
       // One adapter's rows are through: its sums of this chunk.
-      ok = mbar_wait(&done, done_ph, s_abort, g.status, g.budget_ns);
+      ok = mbar_wait(&sh.done, done_ph, s_abort, g.status, g.budget_ns) && ok;
       done_ph ^= 1;
       if (__syncthreads_or(!ok)) break;
       tc_fence_after();
       const bool whole = was.first == __ldg(g.start + was.e) && was.end == __ldg(g.start + was.e + 1);
-      const int mb = warp >> 2, q = warp & 3;
+      const int mb = (warp >> 2) & 1, q = warp & 3;
       const int64_t c = col0 + mb * 128 + q * 32 + lane;
-      const int64_t slot = (int64_t)(chunk + was.e) * g.r * job.C;
+      const int64_t part = (int64_t)(chunk + was.e) * g.r * job.C;
       const int64_t base = (int64_t)was.e * g.r * job.C;
-      for (int k0 = 0; k0 < g.rp; k0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + mb * g.rp + k0, v);
+      for (int k0 = (warp >> 3) * 16; fetcher && k0 < g.rp; k0 += 32) {  // two warps share a quadrant
+        uint32_t v[16], w[16];
+        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + mb * 2 * g.rp + k0;
+        tmem_ld16(at, v);
+        tmem_ld16(at + g.rp, w);
         tmem_wait_ld();
         if (c < job.C)
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             if (k0 + k >= g.r) break;
-            const int64_t at = job.trans ? c * g.r + k0 + k : (int64_t)(k0 + k) * job.C + c;
-            if (whole) ((uint16_t*)job.out)[base + at] = round16(BF16, __uint_as_float(v[k]));
-            else job.partial[slot + at] = __uint_as_float(v[k]);
+            const float sum = __uint_as_float(v[k]) + __uint_as_float(w[k]);
+            const int64_t to = job.trans ? c * g.r + k0 + k : (int64_t)(k0 + k) * job.C + c;
+            if (whole) ((uint16_t*)job.out)[base + to] = round16(BF16, sum);
+            else job.partial[part + to] = sum;
           }
       }
       tc_fence_before();
       __syncthreads();
     }
   }
-  // MMAs still in flight after a wait that gave up end before TMEM is freed.
+  cp_async_wait<0>();
   __syncthreads();
-  if (!ok || *s_abort) {
-    if (t == 0) umma_commit(&done);
-    mbar_wait(&done, done_ph, nullptr, g.status, g.budget_ns);
+  if (*s_abort) {
+    // MMAs still in flight after a wait that gave up end before TMEM is freed.
+    if (t == kOuterFetch) umma_commit(&sh.done);
+    mbar_wait(&sh.done, done_ph, nullptr, g.status, g.budget_ns);
   }
+}
+
+template <bool BF16, int S>
+__global__ void __launch_bounds__(kOuterThreads, 1)
+    k_outer(const __grid_constant__ OuterArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ OuterShared sh;
+  const bool second = (int)blockIdx.x >= g.job[0].tiles;
+  const OuterJob& job = g.job[second];
+  const int64_t col0 = (int64_t)((int)blockIdx.x - (second ? g.job[0].tiles : 0)) * kCols;
+  const int chunk = blockIdx.y;
+  const int total = __ldg(g.start + g.E);
+  const int limit = (chunk + 1) * g.len < total ? (chunk + 1) * g.len : total;
+  if (chunk * g.len >= limit) return;  // the whole CTA: nothing is allocated yet
+  uint32_t cols = 32;
+  while (cols < 4u * g.rp) cols *= 2;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(&sh.empty[i], 1);
+    mbar_init(&sh.done, 1);
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  if (threadIdx.x < 32) tmem_alloc(&sh.tmem, cols);
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  tc_fence_after();
+  if (job.exps) outer_body<BF16, true, S>(g, job, col0, chunk, limit, smem, sh);
+  else outer_body<BF16, false, S>(g, job, col0, chunk, limit, smem, sh);
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x < 32) {
     tc_fence_after();
-    tmem_dealloc(tmem, cols);
+    tmem_dealloc(sh.tmem, cols);
   }
 }
 
@@ -366,10 +439,10 @@ __global__ void k_outer_join(const __grid_constant__ OuterArgs g) {
   }
 }
 
-// Rows per chunk: the most chunks that run at once, two CTAs per SM, each of at
+// Rows per chunk: the most chunks that run at once, one CTA per SM, each of at
 // least 256 rows (a second wave of a few CTAs would double the time).
 int chunk_len(int64_t M, int64_t tiles, int sms) {
-  int64_t chunks = 2 * sms / tiles;
+  int64_t chunks = sms / tiles;
   if (chunks < 1) chunks = 1;
   int64_t len = round_up((M + chunks - 1) / chunks, kStep);
   if (len < 256) len = 256;
@@ -386,6 +459,7 @@ size_t outer_scratch_bytes(int64_t M, int64_t N, int64_t K, int r, int E, int de
   Arena ws(nullptr);
   ws.take((size_t)M * 4);
   ws.take((size_t)(E + 1) * 4);
+  ws.take((size_t)M * 4 * split_half(r));
   ws.take((size_t)(chunks + E) * r * K * 4);
   ws.take((size_t)(chunks + E) * r * N * 4);
   return ws.used;
@@ -413,7 +487,6 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
   b.Z = p.dY;
   b.ldz = p.ldy;
   b.C = p.N;
-  b.L = p.T;
   b.out = p.dB;
   b.trans = 1;
   b.tiles = (int)((p.N + kCols - 1) / kCols);
@@ -425,17 +498,33 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
   Arena ws(scratch);
   int32_t* order = ws.take<int32_t>((size_t)p.M * 4);
   int32_t* start = ws.take<int32_t>((size_t)(p.E + 1) * 4);
+  uint16_t* split = ws.take<uint16_t>((size_t)p.M * 4 * split_half(p.r));
+  b.L = split;
   a.partial = ws.take<float>((size_t)(chunks + p.E) * p.r * p.K * 4);
   b.partial = ws.take<float>((size_t)(chunks + p.E) * p.r * p.N * 4);
   g.order = order;
   g.start = start;
-  k_sort_rows<<<p.E, kSortThreads, 0, stream>>>(p.ids, p.M, p.E, order, start);
+  int64_t more = (p.M * split_half(p.r) + 4 * kSortThreads - 1) / (4 * kSortThreads);
+  if (more > 148) more = 148;
+  k_sort_rows<<<(unsigned)(p.E + more), kSortThreads, 0, stream>>>(p.ids, p.M, p.E, order, start,
+                                                                   p.T, p.r, split, p.bf16);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error("k_sort_rows launch", e);
-  size_t smem = 1024 + 2 * (size_t)(kZBytes + 2 * ((g.rp + 63) / 64) * 8192);
-  if (smem < tmem_share(2 * g.rp)) smem = tmem_share(2 * g.rp);
-  auto kern = p.bf16 ? k_outer<true> : k_outer<false>;
-  int rc = p.bf16 ? allow_smem<k_outer<true>>(smem, dev) : allow_smem<k_outer<false>>(smem, dev);
+  // One CTA per SM: as many stages, up to four, as fit.
+  const int l_bytes = (2 * g.rp + 63) / 64 * 8192;
+  const int stages = l_bytes > 16384 ? 3 : 4;
+  size_t smem = (size_t)stages * (kZBytes + l_bytes);
+  const size_t coded = (size_t)stages * (kZBytes / 2 + l_bytes) + 2 * kZBytes;
+  if (p.exps && smem < coded) smem = coded;
+  smem += 1024;
+  const size_t share = tmem_share(4 * g.rp), most_smem = 224 * 1024;
+  if (smem < share) smem = share < most_smem ? share : most_smem;
+  auto kern = p.bf16 ? (stages == 4 ? k_outer<true, 4> : k_outer<true, 3>)
+                     : (stages == 4 ? k_outer<false, 4> : k_outer<false, 3>);
+  int rc = p.bf16 ? (stages == 4 ? allow_smem<k_outer<true, 4>>(smem, dev)
+                                 : allow_smem<k_outer<true, 3>>(smem, dev))
+                  : (stages == 4 ? allow_smem<k_outer<false, 4>>(smem, dev)
+                                 : allow_smem<k_outer<false, 3>>(smem, dev));
   if (rc) return rc;
   kern<<<dim3((unsigned)tiles, (unsigned)chunks), kOuterThreads, smem, stream>>>(g);
   e = cudaGetLastError();

@@ -130,6 +130,16 @@ __device__ __forceinline__ void ring_drain(uint64_t* full, int stages, int steps
 // ceil(r / 64) blocks of 64.
 __host__ __device__ inline int split_half(int r) { return r <= 32 ? 32 : (r + 63) / 64 * 64; }
 
+// Rounds t to its high and low 16-bit parts and stores them in the split T.
+__device__ __forceinline__ void store_split(uint16_t* split, int64_t row, int half, int c, float t,
+                                            bool bf16) {
+  const uint16_t hi = round16(bf16, t);
+  float rest = t - widen16(bf16, hi);
+  if (!(fabsf(rest) <= 3.0e38f)) rest = 0.0f;  // t not finite: hi says so by itself
+  split[row * 2 * half + c] = hi;
+  split[row * 2 * half + half + c] = round16(bf16, rest);
+}
+
 // ------------------------------------------------- int8 checkpoint codes
 
 constexpr int kGroup = 128;      // columns of a row that share an exponent
