@@ -90,6 +90,26 @@ __device__ __forceinline__ float cluster_sum(uint32_t a, int splits) {
   return s;
 }
 
+__device__ __forceinline__ float4 cluster_sum4(uint32_t a, int splits) {
+  float4 v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    if (q < splits) {
+      uint32_t ra;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(q));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[q].x), "=f"(v[q].y), "=f"(v[q].z), "=f"(v[q].w)
+                   : "r"(ra)
+                   : "memory");
+    }
+  }
+  float4 s = v[0];
+#pragma unroll
+  for (int q = 1; q < 8; ++q)
+    if (q < splits) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
+  return s;
+}
+
 // ---------------------------------------------------------------- k_linear
 //
 // One CTA per 128 x BN tile, or a cluster of CTAs per tile that split the
@@ -263,7 +283,9 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   } else {
-    float* part = (float*)smem;  // [row][BN + 1]
+    // [row][BN + 4]: rows of 16-byte pieces, eight of them across all banks.
+    constexpr int LDP = BN + 4;
+    float* part = (float*)smem;
     if (warp >= 2) {
       const int q = warp & 3;
       const int r = q * 32 + lane;
@@ -275,17 +297,27 @@ __global__ void __launch_bounds__(kThreads)
           tmem_wait_ld();
           if (r < mrows)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) part[r * (BN + 1) + c + i] = __uint_as_float(v[i]);
+            for (int i = 0; i < 32; i += 4)
+              *(uint4*)&part[r * LDP + c + i] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
       }
     }
     cluster_sync();
-    const int share = BN / (int)splits;  // a power of two >= 4
+    const int share = BN / 4 / (int)splits;  // pieces of a row for this CTA
     const int c0 = (int)rank * share;
     for (int e = threadIdx.x; e < mrows * share; e += kThreads) {
-      const int r = e / share, c = c0 + e - r * share;
-      const float s = cluster_sum(smem_u32(&part[r * (BN + 1) + c]), (int)splits);
-      if (col0 + c < g.N) ((uint16_t*)g.Y)[(row0 + r) * g.ldy + col0 + c] = round16(g.bf16, s);
+      const int r = e / share, c = 4 * (c0 + e - r * share);
+      const float4 s = cluster_sum4(smem_u32(&part[r * LDP + c]), (int)splits);
+      const int n = g.N - (col0 + c);
+      uint16_t* y = (uint16_t*)g.Y + (row0 + r) * g.ldy + col0 + c;
+      if (g.y_vec && n >= 4) {
+        *(uint2*)y = make_uint2(pack16(g.bf16, s.x, s.y), pack16(g.bf16, s.z, s.w));
+      } else {
+        if (n > 0) y[0] = round16(g.bf16, s.x);
+        if (n > 1) y[1] = round16(g.bf16, s.y);
+        if (n > 2) y[2] = round16(g.bf16, s.z);
+        if (n > 3) y[3] = round16(g.bf16, s.w);
+      }
     }
     cluster_sync();  // no CTA leaves while a peer reads its partials
   }
@@ -307,22 +339,25 @@ struct LowArgs {
   uint16_t* split;   // [M][2 half], or NULL
   int64_t M;
   int nkb, E, r, rp;  // rp: r rounded up to 16
-  int nacc;           // accumulators that the stages go to in turn
+  int batch;          // adapters of a tile that are multiplied at once
   int bf16;
-  int xstages, astages, xrows;
+  int stages, xrows;
   int32_t* status;
   uint64_t budget_ns;
 };
 
-// T of a tile of 128 rows: each block of 64 contraction elements of X is loaded
-// once and multiplied with the same block of every adapter of the tile, each
-// into its own lanes.  The CTAs of a cluster split the contraction.  Bound by
-// reading X.
-// The tensor cores cut off, rather than round, what a sum's exponent leaves no
-// room for, so the error of a chain of accumulations grows with its length
-// (1.2e-6 of T after 1024 elements, 3.5e-7 after 256).  T is FP32, so the
-// stages go to up to four accumulators in turn, which are added in FP32 at
-// the end.
+// T of a tile of 128 rows, for up to `batch` of the tile's adapters at once,
+// each into TMEM columns of its own; a row then takes its own adapter's.  A
+// stage holds 64 contraction elements of X and of those adapters; a tile with
+// more adapters walks X again for the next ones.  The CTAs of a cluster split
+// the contraction.  Bound by reading X (requests of many rows: one batch).
+//
+// An MMA this narrow lasts some 250 clocks when the next one waits for its
+// sum, so the four steps of 16 elements in a stage go to four accumulators
+// (two from rank 65 on), which are added in FP32 at the end.  That also keeps
+// the chains short: the tensor cores cut off, rather than round, what a sum's
+// exponent leaves no room for, and T was 1.2e-6 off after chains of 1024
+// elements, 3.5e-7 after 256.
 template <bool MNB>
 __global__ void __launch_bounds__(kThreads)
     k_low_rank(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapA,
@@ -332,10 +367,11 @@ __global__ void __launch_bounds__(kThreads)
   const int x_bytes = g.xrows * 128;
   const int a_bytes = MNB ? (g.rp + 63) / 64 * 8192 : g.rp * 128;
   uint8_t* sX = smem;
-  uint8_t* sA = smem + g.xstages * x_bytes;
+  uint8_t* sA = smem + g.stages * x_bytes;
+  float* part = (float*)(sA + g.stages * g.batch * a_bytes);  // [row][rp + 1]
+  const int ldp = g.rp + 1;
   __shared__ SlotList<4> slots;
-  __shared__ uint64_t xfull[kMaxStages], xempty[kMaxStages], afull[kMaxStages], aempty[kMaxStages],
-      done;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, taken;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word;
   volatile int* s_abort = &s_abort_word;
@@ -347,19 +383,17 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t row0 = (int64_t)(blockIdx.x / splits) * kRows;
   const int kb0 = (int)((int64_t)g.nkb * rank / splits);
   const int kb1 = (int)((int64_t)g.nkb * (rank + 1) / splits);
+  const int accs = g.rp <= 64 ? 4 : 2;
   uint32_t cols = 32;
-  while (cols < (uint32_t)(g.rp * g.nacc)) cols *= 2;
+  while (cols < (uint32_t)(accs * g.batch * g.rp)) cols *= 2;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < g.xstages; ++i) {
-      mbar_init(&xfull[i], 1);
-      mbar_init(&xempty[i], 1);
-    }
-    for (int i = 0; i < g.astages; ++i) {
-      mbar_init(&afull[i], 1);
-      mbar_init(&aempty[i], 1);
+    for (int i = 0; i < g.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
     mbar_init(&done, 1);
+    mbar_init(&taken, 4);
     *s_abort = 0;
     fence_mbar_init();
   }
@@ -373,100 +407,105 @@ __global__ void __launch_bounds__(kThreads)
   const int n = slots.n;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      Ring rx(g.xstages), ra(g.astages);
+    if (lane == 0) {
+      Ring rg(g.stages);
       bool ok = true;
-      int ix = 0, ia = 0;
-      for (int kb = kb0; ok && kb < kb1; ++kb) {
-        ok = mbar_wait(&xempty[rx.s], rx.ph ^ 1, s_abort, g.status, g.budget_ns);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&xfull[rx.s], (uint32_t)x_bytes);
-        tma_load_3d(sX + rx.s * x_bytes, &mapX, &xfull[rx.s], kb * kKB, (int)row0, 0);
-        rx.next();
-        ++ix;
-        for (int j = 0; j < n; ++j) {
-          ok = mbar_wait(&aempty[ra.s], ra.ph ^ 1, s_abort, g.status, g.budget_ns);
+      int issued = 0;
+      for (int j0 = 0; ok && j0 < n; j0 += g.batch) {
+        const int cnt = n - j0 < g.batch ? n - j0 : g.batch;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(&empty[rg.s], rg.ph ^ 1, s_abort, g.status, g.budget_ns);
           if (!ok) break;
-          mbar_arrive_expect_tx(&afull[ra.s], (uint32_t)a_bytes);
-          uint8_t* d = sA + ra.s * a_bytes;
-          if constexpr (MNB) {
-            for (int c = 0; c < g.rp; c += 64)
-              tma_load_3d(d + c * 128, &mapA, &afull[ra.s], c, kb * kKB, slots.id[j]);
-          } else {
-            tma_load_3d(d, &mapA, &afull[ra.s], kb * kKB, 0, slots.id[j]);
+          mbar_arrive_expect_tx(&full[rg.s], (uint32_t)(x_bytes + cnt * a_bytes));
+          tma_load_3d(sX + rg.s * x_bytes, &mapX, &full[rg.s], kb * kKB, (int)row0, 0);
+          uint8_t* d = sA + rg.s * g.batch * a_bytes;
+          for (int j = 0; j < cnt; ++j, d += a_bytes) {
+            if constexpr (MNB) {
+              for (int c = 0; c < g.rp; c += 64)
+                tma_load_3d(d + c * 128, &mapA, &full[rg.s], c, kb * kKB, slots.id[j0 + j]);
+            } else {
+              tma_load_3d(d, &mapA, &full[rg.s], kb * kKB, 0, slots.id[j0 + j]);
+            }
           }
-          ra.next();
-          ++ia;
+          rg.next();
+          ++issued;
         }
       }
-      ring_drain(xfull, g.xstages, ix, g.status, g.budget_ns);
-      ring_drain(afull, g.astages, ia, g.status, g.budget_ns);
+      ring_drain(full, g.stages, issued, g.status, g.budget_ns);
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = umma_idesc_16(g.bf16, kRows, g.rp, false, MNB);
-      Ring rx(g.xstages), ra(g.astages);
-      bool ok = n > 0;
-      for (int kb = kb0; ok && kb < kb1; ++kb) {
-        ok = mbar_wait(&xfull[rx.s], rx.ph, s_abort, g.status, g.budget_ns);
+      Ring rg(g.stages);
+      bool ok = true;
+      int batch = 0;
+      for (int j0 = 0; ok && j0 < n; j0 += g.batch, ++batch) {
+        const int cnt = n - j0 < g.batch ? n - j0 : g.batch;
+        if (batch > 0) ok = mbar_wait(&taken, (batch - 1) & 1, s_abort, g.status, g.budget_ns);
         if (!ok) break;
-        const uint32_t x0 = smem_u32(sX + rx.s * x_bytes);
-        const uint32_t d = tmem + (uint32_t)((kb - kb0) % g.nacc * g.rp);
-        const bool more = kb - kb0 >= g.nacc;
-        for (int j = 0; j < n; ++j) {
-          ok = mbar_wait(&afull[ra.s], ra.ph, s_abort, g.status, g.budget_ns);
+        tc_fence_after();
+        // K-major adapters lie side by side: one MMA takes them all.
+        const uint32_t idesc = umma_idesc_16(g.bf16, kRows, MNB ? g.rp : cnt * g.rp, false, MNB);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + ra.s * a_bytes);
+          const uint32_t x0 = smem_u32(sX + rg.s * x_bytes);
+          const uint32_t a0 = smem_u32(sA + rg.s * g.batch * a_bytes);
+          for (int j = 0; j < (MNB ? cnt : 1); ++j)
 #pragma unroll
-          for (int kk = 0; kk < kKB / 16; ++kk)
-            umma_16_masked(d, umma_desc_sw128(x0 + kk * 32),
-                           MNB ? umma_desc_mn128(a0 + kk * 2048, 8192)
-                               : umma_desc_sw128(a0 + kk * 32),
-                           idesc, more || kk != 0, slots.off[j][0], slots.off[j][1],
-                           slots.off[j][2], slots.off[j][3]);
-          umma_commit(&aempty[ra.s]);
-          ra.next();
+            for (int kk = 0; kk < kKB / 16; ++kk) {
+              const uint32_t d = tmem + (uint32_t)(((kk & (accs - 1)) * g.batch + j) * g.rp);
+              umma_bf16(d, umma_desc_sw128(x0 + kk * 32),
+                        MNB ? umma_desc_mn128(a0 + j * a_bytes + kk * 2048, 8192)
+                            : umma_desc_sw128(a0 + kk * 32),
+                        idesc, kb != kb0 || kk >= accs);
+            }
+          umma_commit(&empty[rg.s]);
+          rg.next();
         }
-        if (!ok) break;
-        umma_commit(&xempty[rx.s]);
-        rx.next();
+        umma_commit(&done);
       }
-      umma_commit(&done);
-      mbar_wait(&done, 0, nullptr, g.status, g.budget_ns);
+      // Whatever is in flight ends before TMEM is released.
+      if (!ok) umma_commit(&done);
+      if (n > 0) mbar_wait(&done, (ok ? batch - 1 : batch) & 1, nullptr, g.status, g.budget_ns);
     }
     __syncwarp();
   } else {
-    mbar_wait(&done, 0, nullptr, g.status, g.budget_ns);
-  }
-  __syncthreads();
-  tc_fence_after();
-  const int mrows = g.M - row0 < kRows ? (int)(g.M - row0) : kRows;
-  const int ldp = g.rp + 1;
-  float* part = (float*)smem;
-  if (warp >= 2) {
     const int q = warp & 3;
     const int r = q * 32 + lane;
-    if (q * 32 < mrows)
-      for (int c = 0; c < g.rp; c += 16) {
-        float sum[16];
-        const int used = kb1 - kb0 < g.nacc ? kb1 - kb0 : g.nacc;
-        for (int a = 0; a < used; ++a) {
-          uint32_t v[16];
-          tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + a * g.rp + c, v);
-          tmem_wait_ld();
+    int batch = 0;
+    for (int j0 = 0; j0 < n; j0 += g.batch, ++batch) {
+      const int cnt = n - j0 < g.batch ? n - j0 : g.batch;
+      if (!mbar_wait(&done, batch & 1, s_abort, g.status, g.budget_ns)) break;
+      tc_fence_after();
+      for (int j = 0; j < cnt; ++j) {
+        const uint32_t off = slots.off[j0 + j][q];
+        if (off == ~0u) continue;  // no row of this warp's
+        const bool mine = !((off >> lane) & 1);
+        for (int c = 0; c < g.rp; c += 16) {
+          float sum[16];
+          for (int a = 0; a < accs; ++a) {
+            uint32_t v[16];
+            tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (a * g.batch + j) * g.rp + c, v);
+            tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            sum[i] = a ? sum[i] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
+            for (int i = 0; i < 16; ++i)
+              sum[i] = a ? sum[i] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
+          }
+          if (mine)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) part[r * ldp + c + i] = sum[i];
         }
-        if (r < mrows)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) part[r * ldp + c + i] = sum[i];
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&taken);
+    }
   }
   cluster_sync();
   // Rows of the tile are dealt to the CTAs of the cluster.
+  const int mrows = g.M - row0 < kRows ? (int)(g.M - row0) : kRows;
   const int half = split_half(g.r);
   const int r0 = mrows * (int)rank / (int)splits, r1 = mrows * ((int)rank + 1) / (int)splits;
   for (int e = threadIdx.x; e < (r1 - r0) * half; e += kThreads) {
@@ -640,7 +679,8 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   g.nkb = (int)((p.n_in + kKB - 1) / kKB);
   g.status = status;
   g.budget_ns = wait_budget_ns();
-  if (!p.back && p.M <= 64) {
+  // Few rows (decoding): each may have an adapter of its own.
+  if (!p.back && p.M <= kRows) {
     const int half = split_half(p.r);
     k_low_rank_rows<<<dim3((unsigned)p.M, (unsigned)(half / kLowRanks)), kLowThreads, 0, stream>>>(
         (const uint16_t*)p.X.p, p.X.ld, (const uint16_t*)p.A.p, p.A.ld, p.n_in, g);
@@ -649,22 +689,30 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   }
   g.xrows = p.M >= kRows ? kRows : (int)round_up(p.M, 8);
   const int64_t tiles = (p.M + kRows - 1) / kRows;
+  // Two CTAs per SM at most (a second wave doubles the time), clusters of four
+  // where there are tiles enough (of eight, only 15 fit the GPU at 100 KB of
+  // shared memory a CTA), and chains of at most 512 elements.
+  const int accs = g.rp <= 64 ? 4 : 2;
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * device_sm_count(dev) && g.nkb >= splits * 4)
+  while (splits < (tiles <= 8 ? 8 : 4) && tiles * splits * 2 <= 2 * device_sm_count(dev) &&
+         g.nkb >= splits * 4)
     splits *= 2;
-  // Chains of at most 512 elements where eight CTAs and the accumulators allow it.
-  g.nacc = g.rp <= 64 ? 4 : 2;
-  while (splits < 8 && g.nkb > 8 * splits * g.nacc) splits *= 2;
+  while (splits < 8 && g.nkb > 8 * splits * accs) splits *= 2;
   const int a_bytes = p.back ? (g.rp + 63) / 64 * 8192 : g.rp * 128;
-  g.xstages = 4;
-  g.astages = 4;
-  size_t area = (size_t)g.xstages * g.xrows * 128 + (size_t)g.astages * a_bytes;
-  // The MMA reads 128 rows of X's last stage even if fewer were loaded.
-  const size_t need = (size_t)(g.xstages - 1) * g.xrows * 128 + kRows * 128;
+  // TMEM for two CTAs per SM: 256 columns.
+  g.batch = 256 / (accs * g.rp);
+  if (p.back && g.batch > 2) g.batch = 2;
+  const size_t stage = (size_t)g.xrows * 128 + (size_t)g.batch * a_bytes;
   const size_t red = (size_t)kRows * (g.rp + 1) * 4;
+  const size_t room = (g.rp <= 64 ? 108 : 180) * 1024 - red;
+  g.stages = (int)(room / stage);
+  if (g.stages > 8) g.stages = 8;
+  size_t area = g.stages * stage + red;
+  // (The MMA reads 128 rows of X's last stage even if fewer were loaded: what
+  // lies behind belongs to this CTA.)
+  const size_t need = (size_t)(g.stages - 1) * g.xrows * 128 + kRows * 128;
   if (area < need) area = need;
-  if (area < red) area = red;
-  if (area < tmem_share(g.rp * g.nacc)) area = tmem_share(g.rp * g.nacc);
+  if (area < tmem_share(accs * g.batch * g.rp)) area = tmem_share(accs * g.batch * g.rp);
   CUtensorMap mx, ma;
   int rc;
   if ((rc = make_map(&mx, p.X.p, 2, p.n_in, p.M, 1, p.X.ld * 2, p.X.ld * 2 * p.M, kKB, g.xrows,
@@ -692,7 +740,7 @@ int run_linear_bn(const Product& p, LinearArgs g, const uint16_t* split, int spl
   if (g.stages > kMaxStages) g.stages = kMaxStages;
   size_t area = g.stages * stage;
   const size_t need = (size_t)(g.stages - 1) * g.xrows * 128 + kRows * 128;
-  const size_t red = (size_t)g.xrows * (BN + 1) * 4;
+  const size_t red = (size_t)g.xrows * (BN + 4) * 4;
   if (area < need) area = need;
   if (splits > 1 && area < red) area = red;
   if (area < tmem_share(BN)) area = tmem_share(BN);
@@ -760,15 +808,18 @@ int run_linear(const Product& p, const int32_t* ids, const uint16_t* split, void
     w.status = status;
     return launch_wide(w, dev, stream);
   }
-  const bool few = tiles_m * ((p.n_out + 127) / 128) < sms;
-  const int64_t tiles = tiles_m * ((p.n_out + (few ? 63 : 127)) / (few ? 64 : 128));
+  // 128 columns per CTA; the contraction split over a cluster as long as two
+  // CTAs per SM hold them all (a second wave doubles the time: 64 x 8192 x 4096
+  // took 20 us with 256 CTAs and 30 us with 512).  Full tiles have more to add
+  // up: they are split in four at most, into parts of sixteen stages or more
+  // (1023 x 2048 x 1000 took 17 us whole and 22 us halved, 1777 x 1001 x 2000
+  // 37 us whole and 24 us halved).
+  const int64_t tiles = tiles_m * ((p.n_out + 127) / 128);
+  const int most = p.M > 64 ? 4 : 8, least = p.M > 64 ? 16 : 4;
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * sms && g.nkb >= splits * 4) splits *= 2;
-  if (p.back)
-    return few ? run_linear_bn<64, true>(p, g, split, splits, dev, stream)
-               : run_linear_bn<128, true>(p, g, split, splits, dev, stream);
-  return few ? run_linear_bn<64, false>(p, g, split, splits, dev, stream)
-             : run_linear_bn<128, false>(p, g, split, splits, dev, stream);
+  while (splits < most && tiles * splits * 2 <= 2 * sms && g.nkb >= splits * 2 * least) splits *= 2;
+  return p.back ? run_linear_bn<128, true>(p, g, split, splits, dev, stream)
+                : run_linear_bn<128, false>(p, g, split, splits, dev, stream);
 }
 
 // Copies an operand that TMA cannot read into the workspace, its rows padded

@@ -517,8 +517,7 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
   const size_t coded = (size_t)stages * (kZBytes / 2 + l_bytes) + 2 * kZBytes;
   if (p.exps && smem < coded) smem = coded;
   smem += 1024;
-  const size_t share = tmem_share(4 * g.rp), most_smem = 224 * 1024;
-  if (smem < share) smem = share < most_smem ? share : most_smem;
+  if (smem < tmem_share(4 * g.rp)) smem = tmem_share(4 * g.rp);
   auto kern = p.bf16 ? (stages == 4 ? k_outer<true, 4> : k_outer<true, 3>)
                      : (stages == 4 ? k_outer<false, 4> : k_outer<false, 3>);
   int rc = p.bf16 ? (stages == 4 ? allow_smem<k_outer<true, 4>>(smem, dev)

@@ -278,13 +278,14 @@ int launch_wide(const WideProduct& p, int dev, cudaStream_t stream);
 size_t wide_partial_bytes(int64_t M, int64_t N, int64_t C, int dev);
 
 // Shared memory that a CTA of these kernels asks for at least when it holds
-// `cols` TMEM columns: its share of the SM's 227 KB.  CTAs that fit an SM
-// together then never want more than its 512 columns, so an allocation cannot
+// `cols` TMEM columns: a little more than its share of the SM's 228 KB, less what
+// a CTA has besides (544 columns' shares exceed the SM, 2 x 256's fit).  CTAs that
+// fit an SM together then never want more than its 512 columns, so an allocation cannot
 // block one CTA of a cluster while its peers wait for it.
 inline size_t tmem_share(int cols) {
   int c = 32;
   while (c < cols) c *= 2;
-  return (size_t)c * 456;
+  return (size_t)c * 432;
 }
 
 // Lets kernel K use `bytes` of dynamic shared memory on device dev; the driver
