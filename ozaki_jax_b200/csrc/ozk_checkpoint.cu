@@ -21,6 +21,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
 #include "ozk_tile16.cuh"
 
@@ -47,10 +48,13 @@ struct Elem<OZK_DT_F32> {
   static constexpr int EMAX = 121;
 };
 
+// Larger of two packed pairs of non-negative 16-bit values, NaN if one is.
 template <int DT>
-__device__ __forceinline__ float to_f32(typename Elem<DT>::type u) {
-  if constexpr (DT == OZK_DT_F32) return u;
-  else return widen16(DT == OZK_DT_BF16, u);
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (DT == OZK_DT_BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // Step exponent of a group whose largest magnitude has the FP32 bits `top`.
@@ -75,23 +79,24 @@ __global__ void __launch_bounds__(256)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row0 = (int64_t)blockIdx.y * kTileRows;
   const int64_t col0 = (int64_t)blockIdx.x * kTileCols;
-  float x[kWarpRows][HALVES][VEC];
+  uint32_t x[kWarpRows][HALVES][4];  // 16 bytes of elements
 #pragma unroll
   for (int j = 0; j < kWarpRows; ++j)
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) {
       const int64_t row = row0 + warp * kWarpRows + j;
       const int64_t col = col0 + (h * 32 + lane) * VEC;
+      uint4 q = make_uint4(0, 0, 0, 0);
       if (row < M && vec && col + VEC <= K) {
-        const uint4 q = __ldcs((const uint4*)(X + row * ldx + col));
-        const typename E::type* u = (const typename E::type*)&q;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x[j][h][i] = to_f32<DT>(u[i]);
-      } else {
+        q = __ldcs((const uint4*)(X + row * ldx + col));
+      } else if (row < M) {
+        typename E::type u[VEC] = {};
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-          x[j][h][i] = row < M && col + i < K ? to_f32<DT>(X[row * ldx + col + i]) : 0.0f;
+          if (col + i < K) u[i] = X[row * ldx + col + i];
+        memcpy(&q, u, 16);
       }
+      x[j][h][0] = q.x, x[j][h][1] = q.y, x[j][h][2] = q.z, x[j][h][3] = q.w;
     }
 #pragma unroll
   for (int j = 0; j < kWarpRows; ++j)
@@ -100,34 +105,54 @@ __global__ void __launch_bounds__(256)
       const int r = warp * kWarpRows + j;
       const int64_t row = row0 + r;
       const int64_t col = col0 + (h * 32 + lane) * VEC;
-      uint32_t top = 0;
+      const uint32_t(&w)[4] = x[j][h];
+      // Largest magnitude, NaN if there is one: 16-bit elements two to a word,
+      // FP32 ones as the unsigned integers that they order like.
+      uint32_t top;
+      if constexpr (VEC == 8) {
+        const uint32_t m = 0x7fff7fffu;
+        top = max_pair<DT>(max_pair<DT>(w[0] & m, w[1] & m), max_pair<DT>(w[2] & m, w[3] & m));
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const uint32_t b = __float_as_uint(x[j][h][i]) & 0x7fffffffu;
-        top = b > top ? b : top;
-      }
+        for (int o = LANES / 2; o; o >>= 1) top = max_pair<DT>(top, __shfl_xor_sync(~0u, top, o));
+        const uint32_t hi = __float_as_uint(widen16(DT == OZK_DT_BF16, (uint16_t)(top >> 16)));
+        const uint32_t lo = __float_as_uint(widen16(DT == OZK_DT_BF16, (uint16_t)top));
+        top = max(hi, lo);
+      } else {
+        const uint32_t m = 0x7fffffffu;
+        top = max(max(w[0] & m, w[1] & m), max(w[2] & m, w[3] & m));
 #pragma unroll
-      for (int o = LANES / 2; o; o >>= 1) {
-        const uint32_t b = __shfl_xor_sync(~0u, top, o);
-        top = b > top ? b : top;
+        for (int o = LANES / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
       }
       const int e = group_exponent<DT>(top);
       const float inv = e == kExpNaN ? 0.0f : __uint_as_float((uint32_t)(127 - e) << 23);
+      // x / 2^e is exact; the fused sum with 1.5 2^23 rounds it to the integer
+      // whose two's complement is the low byte.
+      auto element = [&](int i) {
+        if constexpr (VEC == 8) return widen16(DT == OZK_DT_BF16, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
+        else return __uint_as_float(w[i]);
+      };
+      auto low_bytes = [](float a, float b, float c, float d) {
+        return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                           __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+      };
+      constexpr float kRound = 12582912.0f;
       uint32_t q[VEC / 4];
 #pragma unroll
-      for (int i = 0; i < VEC; i += 4) {
-        uint32_t b[4];
+      for (int i = 0; i < VEC; i += 4)
+        q[i / 4] = low_bytes(__fmaf_rn(element(i), inv, kRound), __fmaf_rn(element(i + 1), inv, kRound),
+                             __fmaf_rn(element(i + 2), inv, kRound), __fmaf_rn(element(i + 3), inv, kRound));
+      // A step at the type's upper limit may be too small for the group: those
+      // codes saturate.  (A branch of the warp's, so that no other group pays.)
+      if (__any_sync(~0u, e == E::EMAX) && e == E::EMAX) {
+        auto clamp = [&](float v) { return fminf(fmaxf(v * inv, -127.0f), 127.0f) + kRound; };
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // x / 2^e is exact; the sum with 1.5 2^23 rounds it to the integer
-          // whose two's complement is the low byte.
-          const float v = fminf(fmaxf(x[j][h][i + k] * inv, -127.0f), 127.0f);
-          b[k] = __float_as_uint(__fadd_rn(v, 12582912.0f));
-        }
-        q[i / 4] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040),
-                               0x5410);
-        if (e == kExpNaN) q[i / 4] = 0;
+        for (int i = 0; i < VEC; i += 4)
+          q[i / 4] = low_bytes(clamp(element(i)), clamp(element(i + 1)), clamp(element(i + 2)),
+                               clamp(element(i + 3)));
       }
+      if (e == kExpNaN)
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i) q[i] = 0;
       if (row < M && col < ldc) {
         int8_t* c = codes + row * ldc + col;
         if constexpr (VEC == 8) *(uint2*)c = make_uint2(q[0], q[1]);
@@ -167,8 +192,11 @@ __global__ void __launch_bounds__(256)
       const float s = e[j] == kExpNaN ? __uint_as_float(0x7fc00000u) : pow2f(e[j]);
       float f[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        f[i] = (float)(int8_t)((i < 4 ? q[j].x : q[j].y) >> (8 * (i & 3))) * s;
+      for (int i = 0; i < 8; ++i) {
+        // 2^23 + u is exact in FP32 for the byte u = q + 128
+        const uint32_t u = (i < 4 ? q[j].x : q[j].y) ^ 0x80808080u;
+        f[i] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + (i & 3))) - 8388736.0f) * s;
+      }
       if (vec && col + 8 <= K) {
         __stcs((float4*)o, make_float4(f[0], f[1], f[2], f[3]));
         __stcs((float4*)(o + 4), make_float4(f[4], f[5], f[6], f[7]));
