@@ -4,20 +4,28 @@
 //   back     dX = dY W   (+ U A_i)       W and A_i MN-major
 //   weight   dW = dY^T X^                dY MN-major, X^ from int8 codes
 //
-// Bound by the tensor cores.  Persistent: each CTA pair (cta_group::2, M = 256)
-// walks its tiles; each CTA stages its 128 rows of A and half of B's 256
-// columns per 64 contraction indexes (32 KB), so a stage is read from shared
-// memory at 64 B/clk, half of what the two CTAs would read apart.  Two TMEM
-// accumulators (all 512 columns) let the epilogue of one tile run under the
-// MMAs of the next.
+// Persistent: each CTA pair (cta_group::2, M = 256) walks its tiles; each CTA
+// stages its 128 rows of A and half of B's 256 columns per 64 contraction
+// indexes.  Bound by shared memory: a stage of 4 MMAs lasts 512 clocks on the
+// tensor cores, in which the MMAs read 32 KB of each SM's shared memory and
+// the copies write 32 KB; that is all of its 128 B/clk, and a stage took 714
+// clocks (859 with the converters' traffic).  So where there are tiles enough,
+// a pair takes two tiles one below the other (SUB = 2, 512 x 256) that share
+// B: 112 KB instead of 128 KB for the same work, and in the weight product
+// each code is converted for 512 rows instead of 256.
 //
-// Warps: 0 TMA producer, 1 MMA issuer (one thread of the even CTA), 2-5
-// epilogue, 6 the tile's list of adapters (forward, back) or 6-14 (weight):
-// 6-13 convert each CTA's 128 columns x 64 rows of codes (TMA'd into a ring of
+// SUB = 1: two TMEM accumulators (all 512 columns) let the epilogue of one tile
+// run under the MMAs of the next.  SUB = 2: they belong to the two halves of a
+// tile; the first stages' MMAs into the upper half run while the lower half is
+// still being read.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (one thread of the even CTA), 2-9
+// epilogue, 10 the tile's list of adapters (forward, back) or 10-18 (weight):
+// 10-17 convert each CTA's 128 columns x 64 rows of codes (TMA'd into a ring of
 // their own) into 16-bit values in the MMA's layout, 16 codes per clock and SM
 // at the MMA's full rate, at about 2.5 instructions a code; two groups of four
 // warps take alternate stages, so that a group has two stages' time for its
-// chain of loads, conversions, stores and fence.  Warp 14 turns the exponents
+// chain of loads, conversions, stores and fence.  Warp 18 turns the exponents
 // into 16-bit steps and copies the codes in, some stages ahead of the MMA.  The steps are powers of two, so a code
 // times its step is exact in the operand type and the product is that of the
 // restored matrix.
@@ -36,19 +44,22 @@ constexpr int kTile = 256;
 constexpr int kHalf = 128;       // rows of A, columns of B per CTA
 constexpr int kKB = 64;          // contraction indexes per stage
 constexpr int kABytes = kHalf * kKB * 2;
-constexpr int kStageBytes = 2 * kABytes;
 constexpr int kRawBytes = kHalf * kKB;
 constexpr int kConvWarps = 4;    // of one of the two converter groups
 
-template <WideMode MODE>
+constexpr int kEpiWarps = 8;     // four lane quadrants, two column halves
+constexpr int kWork = 2 + kEpiWarps;  // first warp after the epilogue's
+
+template <WideMode MODE, int SUB>
 struct WideCfg {
   static constexpr bool W = MODE == kWideWeight;
-  static constexpr int STAGES = W ? 5 : 6;
-  static constexpr int RAW = W ? 6 : 0;
-  static constexpr int THREADS = W ? 32 * (7 + 2 * kConvWarps) : 32 * 7;
+  static constexpr int STAGE_BYTES = (SUB + 1) * kABytes;
+  static constexpr int STAGES = SUB == 2 ? 4 : W ? 5 : 6;
+  static constexpr int RAW = W ? (SUB == 2 ? 3 : 6) : 0;
+  static constexpr int THREADS = 32 * (W ? kWork + 2 * kConvWarps + 1 : kWork + 1);
   // All of an SM's shared memory: a CTA holds all TMEM columns, so no other
   // TMEM kernel may share the SM.
-  static constexpr int SMEM = 227 * 1024 - (W ? 3 : 11) * 1024;
+  static constexpr int SMEM = 227 * 1024 - (W ? 3 : SUB == 2 ? 20 : 11) * 1024;
 };
 
 struct WideArgs {
@@ -58,7 +69,8 @@ struct WideArgs {
   int bf16, out_f32, accumulate, o_vec;
   void* out;
   int64_t ldo;
-  float* partial;      // [splits][M][N] when splits > 1
+  float* partial;      // [splits][M][ldp] when splits > 1
+  int64_t ldp;
   const int8_t* exps;  // [groups][C]
   int64_t C;
   const int32_t* ids;
@@ -130,20 +142,21 @@ __device__ __forceinline__ void store_16(uint16_t* o, bool vec, int n, const uin
   }
 }
 
-template <WideMode MODE, bool BF16>
-__global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
+template <WideMode MODE, bool BF16, int SUB>
+__global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
     k_wide(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
            const __grid_constant__ CUtensorMap mapT, const __grid_constant__ CUtensorMap mapBi,
            const __grid_constant__ WideArgs g) {
-  using Cfg = WideCfg<MODE>;
-  constexpr int STAGES = Cfg::STAGES, RAW = Cfg::RAW;
+  using Cfg = WideCfg<MODE, SUB>;
+  constexpr int STAGES = Cfg::STAGES, RAW = Cfg::RAW, kStageBytes = Cfg::STAGE_BYTES;
+  constexpr int kBOff = SUB * kABytes;  // B behind the tile halves of A
   constexpr bool AMN = MODE == kWideWeight, BMN = MODE != kWideForward;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sRaw = smem + STAGES * kStageBytes;
   __shared__ uint64_t full[STAGES], empty[STAGES], rfull[RAW + 1], rempty[RAW + 1], accf[2],
       acce[2], sfull, sempty, done;
-  __shared__ SlotList<MODE == kWideWeight ? 1 : 8> slots;
+  __shared__ SlotList<MODE == kWideWeight ? 1 : 8> slots[SUB];
   __shared__ uint32_t steps[MODE == kWideWeight ? RAW : 1][kKB];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word;
@@ -167,7 +180,7 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&accf[i], 1);
-      mbar_init(&acce[i], 2 * 4);
+      mbar_init(&acce[i], 2 * kEpiWarps);
     }
     mbar_init(&sfull, 1);
     mbar_init(&sempty, rank == 0 ? 2 : 1);
@@ -198,21 +211,28 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
       for (int i = unit; ok && i < items; i += n_units) {
         int tm, tn, sp, kb0, kb1;
         item_at(i, tm, tn, sp, kb0, kb1);
-        const int arow = tm * kTile + (int)rank * kHalf;
+        const int arow = tm * SUB * kTile + (int)rank * kHalf;
         const int bcol = tn * kTile + (int)rank * kHalf;
-        auto load = [&](const CUtensorMap* ma, int ax, const CUtensorMap* mb, int bx, int bz) {
+        // The halves [s0, s1) of A at contraction index ax, and B.
+        auto load = [&](const CUtensorMap* ma, int ax, int s0, int s1, const CUtensorMap* mb, int bx,
+                        int bz) {
           if (!mbar_wait(&empty[rg.s], rg.ph ^ 1, s_abort, g.status, g.budget_ns)) return false;
           if (rank == 0)
-            mbar_arrive_expect_tx(&full[rg.s], 2 * (MODE == kWideWeight ? kABytes : kStageBytes));
+            mbar_arrive_expect_tx(&full[rg.s],
+                                  2 * (s1 - s0 + (MODE == kWideWeight ? 0 : 1)) * kABytes);
           const uint32_t fb = mapa_u32(&full[rg.s], 0);
-          uint8_t* a = smem + rg.s * kStageBytes;
-          uint8_t* b = a + kABytes;
-          if constexpr (AMN) {
-            tma_load_3d_pair(a, ma, fb, arow, ax, 0);
-            tma_load_3d_pair(a + 8192, ma, fb, arow + 64, ax, 0);
-          } else {
-            tma_load_3d_pair(a, ma, fb, ax, arow, 0);
+          uint8_t* st = smem + rg.s * kStageBytes;
+          for (int s = s0; s < s1; ++s) {
+            uint8_t* a = st + s * kABytes;
+            const int row = arow + s * kTile;
+            if constexpr (AMN) {
+              tma_load_3d_pair(a, ma, fb, row, ax, 0);
+              tma_load_3d_pair(a + 8192, ma, fb, row + 64, ax, 0);
+            } else {
+              tma_load_3d_pair(a, ma, fb, ax, row, 0);
+            }
           }
+          uint8_t* b = st + kBOff;
           if constexpr (MODE == kWideForward) {
             tma_load_3d_pair(b, mb, fb, bx, bcol, bz);
           } else if constexpr (MODE == kWideBack) {
@@ -223,16 +243,16 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
           ++issued;
           return true;
         };
-        for (int kb = kb0; ok && kb < kb1; ++kb) ok = load(&mapA, kb * kKB, &mapB, kb * kKB, 0);
+        for (int kb = kb0; ok && kb < kb1; ++kb) ok = load(&mapA, kb * kKB, 0, SUB, &mapB, kb * kKB, 0);
         if (MODE != kWideWeight && g.r > 0) {
           if (!waited) grid_wait();  // the split T comes from the kernel before this one
           waited = true;
           ok = ok && mbar_wait(&sfull, sph, s_abort, g.status, g.budget_ns);
-          const int n = ok ? slots.n : 0;
-          for (int j = 0; ok && j < n; ++j)
-            for (int b = 0; ok && b < blocks; ++b)
-              ok = load(&mapT, blocks == 1 ? 0 : (b & 1) * half + (b >> 1) * 64, &mapBi,
-                        blocks == 1 ? 0 : (b >> 1) * 64, slots.id[j]);
+          for (int s = 0; ok && s < SUB; ++s)
+            for (int j = 0; ok && j < slots[s].n; ++j)
+              for (int b = 0; ok && b < blocks; ++b)
+                ok = load(&mapT, blocks == 1 ? 0 : (b & 1) * half + (b >> 1) * 64, s, s + 1, &mapBi,
+                          blocks == 1 ? 0 : (b >> 1) * 64, slots[s].id[j]);
           if (ok) mbar_arrive(&sempty);
           sph ^= 1;
         }
@@ -256,95 +276,133 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
       auto desc_b = [](uint32_t b, int kk) {
         return BMN ? umma_desc_mn128(b + kk * 2048, 8192) : umma_desc_sw128(b + kk * 32);
       };
-      for (int i = unit; ok && i < items; i += n_units, ++it) {
+      // One stage's MMAs into accumulator `buf` from half s of A.
+      auto multiply = [&](int slot, int s, int buf, bool fresh) {
+        const uint32_t a0 = smem_u32(smem + slot * kStageBytes) + s * kABytes;
+        const uint32_t b0 = smem_u32(smem + slot * kStageBytes) + kBOff;
+#pragma unroll
+        for (int kk = 0; kk < kKB / 16; ++kk)
+          umma_bf16_pair(tmem + buf * kTile, desc_a(a0, kk), desc_b(b0, kk), idesc, !fresh || kk != 0);
+      };
+      auto free_acc = [&](int buf, uint32_t parity) {
+        const bool k = mbar_wait(&acce[buf], parity, s_abort, g.status, g.budget_ns);
+        tc_fence_after();
+        return k;
+      };
+      for (int i = unit; ok && i < items; i += n_units) {
         int tm, tn, sp, kb0, kb1;
         item_at(i, tm, tn, sp, kb0, kb1);
-        int buf = it & 1;
-        uint32_t d = tmem + buf * kTile;
-        int head = kb0;  // first stage of this accumulator's chain
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (kb == kb0 || kb - head == g.chain) {
-            if (kb != kb0) {
-              umma_commit_pair(&accf[buf], 0x3);
+        int buf = 0;
+        if constexpr (SUB == 1) {
+          int head = kb0;  // first stage of this accumulator's chain
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (kb == kb0 || kb - head == g.chain) {
+              if (kb != kb0) umma_commit_pair(&accf[buf], 0x3);
+              buf = it & 1;
+              head = kb;
+              if (!(ok = free_acc(buf, ((it >> 1) & 1) ^ 1))) break;
               ++it;
             }
-            buf = it & 1;
-            d = tmem + buf * kTile;
-            head = kb;
-            ok = mbar_wait(&acce[buf], ((it >> 1) & 1) ^ 1, s_abort, g.status, g.budget_ns);
+            ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
             if (!ok) break;
             tc_fence_after();
+            multiply(rg.s, 0, buf, kb == head);
+            umma_commit_pair(&empty[rg.s], 0x3);
+            rg.next();
           }
-          ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + rg.s * kStageBytes), b0 = a0 + kABytes;
-#pragma unroll
-          for (int kk = 0; kk < kKB / 16; ++kk)
-            umma_bf16_pair(d, desc_a(a0, kk), desc_b(b0, kk), idesc, kb != head || kk != 0);
-          umma_commit_pair(&empty[rg.s], 0x3);
-          rg.next();
+        } else {
+          // The upper half's MMAs of the first stages, as many as the ring
+          // holds, while the epilogue still reads the lower half.
+          const int first = kb1 - kb0 < STAGES ? kb1 - kb0 : STAGES;
+          if (!(ok = free_acc(0, (it & 1) ^ 1))) break;
+          Ring low = rg;
+          for (int k = 0; k < first; ++k) {
+            ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
+            if (!ok) break;
+            tc_fence_after();
+            multiply(rg.s, 0, 0, k == 0);
+            rg.next();
+          }
+          if (!ok || !(ok = free_acc(1, (it & 1) ^ 1))) break;
+          for (int k = 0; k < first; ++k) {
+            multiply(low.s, 1, 1, k == 0);
+            umma_commit_pair(&empty[low.s], 0x3);
+            low.next();
+          }
+          for (int kb = kb0 + first; kb < kb1; ++kb) {
+            ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
+            if (!ok) break;
+            tc_fence_after();
+            multiply(rg.s, 0, 0, false);
+            multiply(rg.s, 1, 1, false);
+            umma_commit_pair(&empty[rg.s], 0x3);
+            rg.next();
+          }
+          ++it;
         }
         if constexpr (MODE != kWideWeight) {
           if (g.r > 0) {
             ok = ok && mbar_wait(&sfull, sph, s_abort, g.status, g.budget_ns);
-            const int n = ok ? slots.n : 0;
-            for (int j = 0; ok && j < n; ++j) {
-              uint32_t off[8];
+            for (int s = 0; ok && s < SUB; ++s) {
+              const uint32_t d = tmem + (SUB == 1 ? buf : s) * kTile;
+              for (int j = 0; ok && j < slots[s].n; ++j) {
+                uint32_t off[8];
 #pragma unroll
-              for (int w = 0; w < 8; ++w) off[w] = slots.off[j][w];
-              for (int b = 0; b < blocks; ++b) {
-                ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t a0 = smem_u32(smem + rg.s * kStageBytes), b0 = a0 + kABytes;
-                const int left = g.r - (b >> 1) * 64;
-                const int steps = left >= 64 ? 4 : (left + 15) / 16;
-                for (int kk = 0; kk < steps; ++kk) {
-                  umma_16_masked_pair(d, desc_a(a0, kk), desc_b(b0, kk), idesc, 1, off);
-                  if (blocks == 1)
-                    umma_16_masked_pair(d, umma_desc_sw128(a0 + 64 + kk * 32), desc_b(b0, kk),
-                                        idesc, 1, off);
+                for (int w = 0; w < 8; ++w) off[w] = slots[s].off[j][w];
+                for (int b = 0; b < blocks; ++b) {
+                  ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
+                  if (!ok) break;
+                  tc_fence_after();
+                  const uint32_t a0 = smem_u32(smem + rg.s * kStageBytes) + s * kABytes;
+                  const uint32_t b0 = smem_u32(smem + rg.s * kStageBytes) + kBOff;
+                  const int left = g.r - (b >> 1) * 64;
+                  const int steps = left >= 64 ? 4 : (left + 15) / 16;
+                  for (int kk = 0; kk < steps; ++kk) {
+                    umma_16_masked_pair(d, desc_a(a0, kk), desc_b(b0, kk), idesc, 1, off);
+                    if (blocks == 1)
+                      umma_16_masked_pair(d, umma_desc_sw128(a0 + 64 + kk * 32), desc_b(b0, kk),
+                                          idesc, 1, off);
+                  }
+                  umma_commit_pair(&empty[rg.s], 0x3);
+                  rg.next();
                 }
-                umma_commit_pair(&empty[rg.s], 0x3);
-                rg.next();
               }
+              if (SUB == 2 && ok) umma_commit_pair(&accf[s], 0x3);
             }
             if (ok) mbar_arrive(&sempty);
             sph ^= 1;
           }
         }
         if (!ok) break;
-        umma_commit_pair(&accf[buf], 0x3);
+        if (SUB == 1) {
+          umma_commit_pair(&accf[buf], 0x3);
+        } else if (MODE == kWideWeight || g.r == 0) {
+          umma_commit_pair(&accf[0], 0x3);
+          umma_commit_pair(&accf[1], 0x3);
+        }
       }
       umma_commit_pair(&done, 0x1);
       mbar_wait(&done, 0, nullptr, g.status, g.budget_ns);
     }
     __syncwarp();
-  } else if (warp < 6) {
+  } else if (warp < kWork) {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;
+    const int q = warp & 3, cbeg = (warp - 2) / 4 * (kTile / 2);
     int it = 0;
     bool ok = true;
-    for (int i = unit; ok && i < items; i += n_units) {
-      int tm, tn, sp, kb0, kb1;
-      item_at(i, tm, tn, sp, kb0, kb1);
-      for (int head = kb0; head < kb1; head += g.chain, ++it) {
-      const int buf = it & 1;
-      ok = mbar_wait(&accf[buf], (it >> 1) & 1, s_abort, g.status, g.budget_ns);
-      if (!ok) break;
-      const bool add = head != kb0;  // this thread wrote the sum so far
+    auto drain = [&](int buf, uint32_t parity, int64_t row0, int tn, int sp, bool add) {
+      if (!mbar_wait(&accf[buf], parity, s_abort, g.status, g.budget_ns)) return false;
       tc_fence_after();
-      const int64_t row = (int64_t)tm * kTile + rank * kHalf + q * 32 + lane;
-      const int64_t col0 = (int64_t)tn * kTile;
-      const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + buf * kTile;
+      const int64_t row = row0 + rank * kHalf + q * 32 + lane;
+      const int64_t col0 = (int64_t)tn * kTile + cbeg;
+      const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + buf * kTile + cbeg;
 #pragma unroll 1
-      for (int c = 0; c < kTile; c += 32) {
+      for (int c = 0; c < kTile / 2; c += 32) {
         uint32_t v[32];
         tmem_ld32(acc + c, v);
         tmem_wait_ld();
-        if (c == kTile - 32) {
-          // The accumulator is read: the tile after the next may start.
+        if (c == kTile / 2 - 32) {
+          // This half of the accumulator is read.
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_u32(&acce[buf], 0));
@@ -352,19 +410,30 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
         const int64_t left = g.N - (col0 + c);
         if (row >= g.M || left <= 0) continue;
         const int n = left < 32 ? (int)left : 32;
-        if (g.splits > 1) {
-          store_f32(g.partial + ((int64_t)sp * g.M + row) * g.N + col0 + c, (g.N & 3) == 0, n, v,
-                    add);
-        } else if (g.out_f32) {
+        if (g.splits > 1)
+          store_f32(g.partial + ((int64_t)sp * g.M + row) * g.ldp + col0 + c, true, n, v, add);
+        else if (g.out_f32)
           store_f32((float*)g.out + row * g.ldo + col0 + c, g.o_vec, n, v, add || g.accumulate);
-        } else {
+        else
           store_16((uint16_t*)g.out + row * g.ldo + col0 + c, g.o_vec, n, v, g.accumulate, BF16);
-        }
       }
+      return true;
+    };
+    for (int i = unit; ok && i < items; i += n_units) {
+      int tm, tn, sp, kb0, kb1;
+      item_at(i, tm, tn, sp, kb0, kb1);
+      const int64_t row0 = (int64_t)tm * SUB * kTile;
+      if constexpr (SUB == 1) {
+        // (Each thread adds to sums that it has written itself.)
+        for (int head = kb0; ok && head < kb1; head += g.chain, ++it)
+          ok = drain(it & 1, (it >> 1) & 1, row0, tn, sp, head != kb0);
+      } else {
+        for (int s = 0; ok && s < 2; ++s) ok = drain(s, it & 1, row0 + s * kTile, tn, sp, false);
+        ++it;
       }
     }
   } else if constexpr (MODE == kWideWeight) {
-    if (warp == 6 + 2 * kConvWarps) {
+    if (warp == kWork + 2 * kConvWarps) {
       // ------------------------------------------- codes' copies and steps
       Ring rr(RAW);
       bool ok = true;
@@ -412,10 +481,10 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
       // ---------------------------------------------------------- converters
       // Thread: rows t / 16 + 8 j of the stage, 8 columns at 8 (t % 16); lanes
       // of a half warp write one row's 16-byte pieces, eight to a 128-byte line.
-      const int cg = (warp - 6) / kConvWarps;  // converter group
-      const int t = (threadIdx.x - 192) % (32 * kConvWarps);
+      const int cg = (warp - kWork) / kConvWarps;  // converter group
+      const int t = (threadIdx.x - 32 * kWork) % (32 * kConvWarps);
       const int piece = t & 15, r0 = t >> 4;
-      const uint32_t to = smem_u32(smem) + kABytes + (piece >> 3) * 8192;
+      const uint32_t to = smem_u32(smem) + kBOff + (piece >> 3) * 8192;
       Ring rg(STAGES), rr(RAW);
       bool ok = true;
       int turn = 0;
@@ -461,7 +530,9 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
       int tm, tn, sp, kb0, kb1;
       item_at(i, tm, tn, sp, kb0, kb1);
       if (!mbar_wait(&sempty, ph ^ 1, s_abort, g.status, g.budget_ns)) break;
-      build_slots<8>(g.ids, (int64_t)tm * kTile, g.M, g.E, (SlotList<8>*)(void*)&slots, lane);
+      for (int s = 0; s < SUB; ++s)
+        build_slots<8>(g.ids, ((int64_t)tm * SUB + s) * kTile, g.M, g.E,
+                       (SlotList<8>*)(void*)&slots[s], lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sfull);
       ph ^= 1;
@@ -476,14 +547,14 @@ __global__ void __launch_bounds__(WideCfg<MODE>::THREADS, 1)
 }
 
 // Sum of the contraction's parts, in order, into the output.
-__global__ void k_wide_join(const float* part, int splits, int64_t M, int64_t N, void* out,
-                            int64_t ldo, int out_f32, int bf16, int accumulate) {
+__global__ void k_wide_join(const float* part, int splits, int64_t M, int64_t N, int64_t ldp,
+                            void* out, int64_t ldo, int out_f32, int bf16, int accumulate) {
   const int64_t n = M * N;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
        i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / N, c = i - r * N, at = r * ldo + c;
     float s = 0.0f;
-    for (int q = 0; q < splits; ++q) s += part[q * n + i];
-    const int64_t r = i / N, at = r * ldo + (i - r * N);
+    for (int q = 0; q < splits; ++q) s += part[(q * M + r) * ldp + c];
     if (out_f32) {
       float* o = (float*)out + at;
       *o = s + (accumulate ? *o : 0.0f);
@@ -505,9 +576,9 @@ int wide_splits(int64_t M, int64_t N, int64_t C, int dev) {
   return s < 2 ? 1 : (int)s;
 }
 
-template <WideMode MODE>
+template <WideMode MODE, int SUB>
 int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) {
-  using Cfg = WideCfg<MODE>;
+  using Cfg = WideCfg<MODE, SUB>;
   CUtensorMap ma, mb, mt, mbi;
   memset(&mt, 0, sizeof(mt));
   memset(&mbi, 0, sizeof(mbi));
@@ -535,9 +606,9 @@ int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) 
       rc = make_map(&mbi, p.Bi, 2, p.N, p.r, p.E, p.ldbi * 2, p.ldbi * 2 * p.r, 64, 64, true);
     if (rc) return rc;
   }
-  auto kern = p.bf16 ? k_wide<MODE, true> : k_wide<MODE, false>;
-  if ((rc = p.bf16 ? allow_smem<k_wide<MODE, true>>(Cfg::SMEM, dev)
-                   : allow_smem<k_wide<MODE, false>>(Cfg::SMEM, dev)))
+  auto kern = p.bf16 ? k_wide<MODE, true, SUB> : k_wide<MODE, false, SUB>;
+  if ((rc = p.bf16 ? allow_smem<k_wide<MODE, true, SUB>>(Cfg::SMEM, dev)
+                   : allow_smem<k_wide<MODE, false, SUB>>(Cfg::SMEM, dev)))
     return rc;
   const int items = g.tiles_m * g.tiles_n * g.splits;
   const int units = device_sm_count(dev) / 2;
@@ -563,7 +634,7 @@ int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) 
 
 size_t wide_partial_bytes(int64_t M, int64_t N, int64_t C, int dev) {
   const int s = wide_splits(M, N, C, dev);
-  return s > 1 ? (size_t)s * M * N * 4 : 0;
+  return s > 1 ? (size_t)s * M * round_up(N, 4) * 4 : 0;
 }
 
 int launch_wide(const WideProduct& p, int dev, cudaStream_t stream) {
@@ -590,20 +661,37 @@ int launch_wide(const WideProduct& p, int dev, cudaStream_t stream) {
   g.ldo = p.ldo;
   g.o_vec = ((uintptr_t)p.out & 15) == 0 && p.ldo % (p.out_f32 ? 4 : 8) == 0;
   g.partial = p.partial;
+  g.ldp = round_up(p.N, 4);
   g.exps = p.exps;
   g.ids = p.ids;
   g.r = p.r;
   g.E = p.E;
   g.status = p.status;
   g.budget_ns = wait_budget_ns();
-  int rc = p.mode == kWideForward ? launch_mode<kWideForward>(p, g, dev, stream)
-           : p.mode == kWideBack  ? launch_mode<kWideBack>(p, g, dev, stream)
-                                  : launch_mode<kWideWeight>(p, g, dev, stream);
+  // Two tiles at once where that does not leave more CTA pairs idle in the last
+  // round (a round of double tiles lasts 1.7 of a round of single ones).  FP32
+  // results change accumulators every 1024 indexes, which only single tiles do
+  // without a pause.
+  const int units = device_sm_count(dev) / 2;
+  const int64_t one = (tm * tn + units - 1) / units;
+  const int64_t two = ((p.M + 2 * kTile - 1) / (2 * kTile) * tn + units - 1) / units;
+  const bool twice = g.splits == 1 && !p.out_f32 && 17 * two <= 10 * one;
+  if (twice) g.tiles_m = (int)((p.M + 2 * kTile - 1) / (2 * kTile));
+  int rc;
+  if (p.mode == kWideForward)
+    rc = twice ? launch_mode<kWideForward, 2>(p, g, dev, stream)
+               : launch_mode<kWideForward, 1>(p, g, dev, stream);
+  else if (p.mode == kWideBack)
+    rc = twice ? launch_mode<kWideBack, 2>(p, g, dev, stream)
+               : launch_mode<kWideBack, 1>(p, g, dev, stream);
+  else
+    rc = twice ? launch_mode<kWideWeight, 2>(p, g, dev, stream)
+               : launch_mode<kWideWeight, 1>(p, g, dev, stream);
   if (rc || g.splits == 1) return rc;
   int64_t blocks = (p.M * p.N + 255) / 256;
   if (blocks > 148 * 8) blocks = 148 * 8;
-  k_wide_join<<<(unsigned)blocks, 256, 0, stream>>>(p.partial, g.splits, p.M, p.N, p.out, p.ldo,
-                                                    p.out_f32, p.bf16, p.accumulate);
+  k_wide_join<<<(unsigned)blocks, 256, 0, stream>>>(p.partial, g.splits, p.M, p.N, g.ldp, p.out,
+                                                    p.ldo, p.out_f32, p.bf16, p.accumulate);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? OZK_OK : set_cuda_error("k_wide_join launch", e);
 }
