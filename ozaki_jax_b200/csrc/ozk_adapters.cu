@@ -69,27 +69,9 @@ __device__ __forceinline__ void store_cols(void* Y, int64_t at, const uint32_t* 
   }
 }
 
-// Sum over the CTAs of the cluster (at most 8), in rank order, of the FP32
-// partial at shared-memory address `a` of each.  The loads are independent, so
+// Sum over the CTAs of the cluster (at most 8), in rank order, of the four FP32
+// partials at shared-memory address `a` of each.  The loads are independent, so
 // their round trips overlap.
-__device__ __forceinline__ float cluster_sum(uint32_t a, int splits) {
-  float v[8];
-#pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    v[q] = 0.0f;
-    if (q < splits) {
-      uint32_t ra;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(q));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[q]) : "r"(ra) : "memory");
-    }
-  }
-  float s = v[0];
-#pragma unroll
-  for (int q = 1; q < 8; ++q)
-    if (q < splits) s += v[q];
-  return s;
-}
-
 __device__ __forceinline__ float4 cluster_sum4(uint32_t a, int splits) {
   float4 v[8];
 #pragma unroll
@@ -368,8 +350,8 @@ __global__ void __launch_bounds__(kThreads)
   const int a_bytes = MNB ? (g.rp + 63) / 64 * 8192 : g.rp * 128;
   uint8_t* sX = smem;
   uint8_t* sA = smem + g.stages * x_bytes;
-  float* part = (float*)(sA + g.stages * g.batch * a_bytes);  // [row][rp + 1]
-  const int ldp = g.rp + 1;
+  float* part = (float*)(sA + g.stages * g.batch * a_bytes);  // [row][rp + 4], in 16-byte pieces
+  const int ldp = g.rp + 4;
   __shared__ SlotList<4> slots;
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, taken;
   __shared__ uint32_t s_tmem;
@@ -484,18 +466,23 @@ __global__ void __launch_bounds__(kThreads)
         if (off == ~0u) continue;  // no row of this warp's
         const bool mine = !((off >> lane) & 1);
         for (int c = 0; c < g.rp; c += 16) {
-          float sum[16];
-          for (int a = 0; a < accs; ++a) {
-            uint32_t v[16];
-            tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (a * g.batch + j) * g.rp + c, v);
-            tmem_wait_ld();
+          uint32_t v[4][16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              sum[i] = a ? sum[i] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
+          for (int a = 0; a < 4; ++a)
+            if (a < accs)
+              tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (a * g.batch + j) * g.rp + c, v[a]);
+          tmem_wait_ld();
+          float sum[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sum[i] = __uint_as_float(v[0][i]) + __uint_as_float(v[1][i]);
+            if (accs == 4) sum[i] += __uint_as_float(v[2][i]) + __uint_as_float(v[3][i]);
           }
           if (mine)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) part[r * ldp + c + i] = sum[i];
+            for (int i = 0; i < 16; i += 4)
+              *(float4*)&part[r * ldp + c + i] =
+                  make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
         }
       }
       tc_fence_before();
@@ -508,16 +495,31 @@ __global__ void __launch_bounds__(kThreads)
   const int mrows = g.M - row0 < kRows ? (int)(g.M - row0) : kRows;
   const int half = split_half(g.r);
   const int r0 = mrows * (int)rank / (int)splits, r1 = mrows * ((int)rank + 1) / (int)splits;
-  for (int e = threadIdx.x; e < (r1 - r0) * half; e += kThreads) {
-    const int r = r0 + e / half, c = e % half;
+  for (int e = threadIdx.x; e < (r1 - r0) * (half / 4); e += kThreads) {
+    const int r = r0 + e / (half / 4), c = e % (half / 4) * 4;
     const int64_t row = row0 + r;
-    float t = 0.0f;
+    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const int i = row_adapter(g.ids, row, g.M, g.E);
-    if (i >= 0 && c < g.r)
-      t = cluster_sum(smem_u32(&part[r * ldp + c]), (int)splits) *
-          (g.scale ? g.alpha * g.scale[i] : g.alpha);
-    if (g.low && c < g.r) g.low[row * g.r + c] = t;
-    if (g.split) store_split(g.split, row, half, c, t, g.bf16);
+    if (i >= 0 && c < g.r) {  // (columns r to rp of the sums are zero)
+      t = cluster_sum4(smem_u32(&part[r * ldp + c]), (int)splits);
+      const float f = g.scale ? g.alpha * g.scale[i] : g.alpha;
+      t.x *= f, t.y *= f, t.z *= f, t.w *= f;
+    }
+    if (g.low) {
+      float* o = g.low + row * g.r + c;
+      if (c < g.r) o[0] = t.x;
+      if (c + 1 < g.r) o[1] = t.y;
+      if (c + 2 < g.r) o[2] = t.z;
+      if (c + 3 < g.r) o[3] = t.w;
+    }
+    if (g.split) {
+      uint32_t hi[2], lo[2];
+      split16(g.bf16, t.x, t.y, hi[0], lo[0]);
+      split16(g.bf16, t.z, t.w, hi[1], lo[1]);
+      uint16_t* o = g.split + row * 2 * half + c;
+      *(uint2*)o = make_uint2(hi[0], hi[1]);
+      *(uint2*)(o + half) = make_uint2(lo[0], lo[1]);
+    }
   }
   cluster_sync();
   tc_fence_before();
@@ -703,7 +705,7 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   g.batch = 256 / (accs * g.rp);
   if (p.back && g.batch > 2) g.batch = 2;
   const size_t stage = (size_t)g.xrows * 128 + (size_t)g.batch * a_bytes;
-  const size_t red = (size_t)kRows * (g.rp + 1) * 4;
+  const size_t red = (size_t)kRows * (g.rp + 4) * 4;
   const size_t room = (g.rp <= 64 ? 108 : 180) * 1024 - red;
   g.stages = (int)(room / stage);
   if (g.stages > 8) g.stages = 8;

@@ -39,7 +39,6 @@ constexpr int kOuterThreads = kOuterFetch + 64;
 constexpr int kCols = 256;       // columns of Z per CTA: two accumulators of 128
 constexpr int kStep = 64;        // rows per stage
 constexpr int kZBytes = kCols * kStep * 2;
-constexpr int kZRows = kStep / kOuterWarps;  // rows of a stage that a warp fetches
 
 // order: the rows of adapters 0, 1, ... in turn, each adapter's in ascending
 // order; start[e]: the first place of adapter e.
@@ -149,10 +148,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -208,8 +203,13 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
     }
     ahead.next(g.start, g.E, limit);
   };
-  const int64_t col = col0 + lane * 8;
-  const uint32_t swz = (uint32_t)(lane & 7) << 4;  // this lane's piece of a 128-byte line
+  // A thread fetches 16 bytes of each of FETCH rows: 8 columns of four rows, a
+  // warp a row; or 16 codes of two rows, a half warp a row.
+  constexpr int FETCH = CODES ? 2 : 4;
+  const int row0 = CODES ? 2 * warp + (lane >> 4) : warp;
+  constexpr int ROW_STEP = CODES ? 2 * kOuterWarps : kOuterWarps;
+  const int at_col = CODES ? (lane & 15) * 16 : lane * 8;
+  const int64_t col = col0 + at_col;
   // This thread's 16-byte pieces of L's parts: the row, where it comes from in
   // that row, where it goes in a stage.
   const int lp = g.rp / 8, pieces = 2 * kStep * lp;
@@ -227,28 +227,29 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
   // What does not change from stage to stage: this lane's bytes of a row of Z
   // (its 8 columns, or those of them inside the matrix) and where they go.
   const int64_t left = (CODES ? job.ldz : job.C) - col;
-  const uint32_t z_bytes = left <= 0 ? 0 : CODES ? 8 : left < 8 ? 2 * (uint32_t)left : 16;
+  const uint32_t z_bytes = left <= 0 ? 0 : CODES ? 16 : left < 8 ? 2 * (uint32_t)left : 16;
   const int64_t z_pitch = job.ldz * (CODES ? 1 : 2);
   const char* z_from = (const char*)job.Z + (z_bytes ? col * (CODES ? 1 : 2) : 0);
   const bool vec = CODES || job.vec;
-  uint32_t z_to[kZRows];
+  // Where 8 columns of row r belong in the MMA's layout.
+  auto place = [](int r, int c) {
+    return (uint32_t)((c >> 6) * 8192 + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4));
+  };
+  uint32_t z_to[FETCH];
 #pragma unroll
-  for (int j = 0; j < kZRows; ++j) {
-    const int r = warp + kOuterWarps * j;
-    z_to[j] = CODES ? r * 256 + lane * 8
-                    : (lane >> 3) * 8192 + r * 128 + (swz ^ ((uint32_t)(r & 7) << 4));
+  for (int j = 0; j < FETCH; ++j) {
+    const int r = row0 + ROW_STEP * j;
+    z_to[j] = CODES ? r * 256 + at_col : place(r, at_col);
   }
   const char* l_base = (const char*)job.L;
   const int l_pitch = 4 * half;
   auto load = [&](uint32_t zb, const int* rows) {
 #pragma unroll
-    for (int j = 0; j < kZRows; ++j) {
-      const int row = rows[warp + kOuterWarps * j];
+    for (int j = 0; j < FETCH; ++j) {
+      const int row = rows[row0 + ROW_STEP * j];
       const char* p = z_from + (row >= 0 ? row : 0) * z_pitch;
       const uint32_t n = row >= 0 ? z_bytes : 0;
-      if constexpr (CODES) {
-        cp_async8(zb + z_to[j], p, n);
-      } else if (vec) {
+      if (vec) {
         cp_async16(zb + z_to[j], p, n);
       } else {
         const uint16_t* e = (const uint16_t*)p;
@@ -269,12 +270,13 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
                  row >= 0 ? 16 : 0);
     }
   };
-  // Steps of a stage: lane 4 g + j holds row warp + 16 j of column group g.
-  // (Turned into 16-bit steps when they are used, an iteration later.)
+  // Exponents of a stage: lane 4 j + 2 h + g holds row row0 + 32 j of half warp h
+  // in column group g.  (Turned into 16-bit steps when they are used, an
+  // iteration later.)
   auto exponents = [&](int stage) {
-    if (!CODES || !fetcher || lane >= 2 * kZRows) return 0;
-    const int row = sh.rows[stage % kRowSlots][warp + kOuterWarps * (lane % kZRows)];
-    const int64_t group = col0 / kGroup + lane / kZRows;
+    if (!CODES || !fetcher || lane >= 8) return 0;
+    const int row = sh.rows[stage % kRowSlots][2 * warp + (lane >> 1 & 1) + ROW_STEP * (lane >> 2)];
+    const int64_t group = col0 / kGroup + (lane & 1);
     return row >= 0 && group * kGroup < job.ldz ? (int)__ldg(job.exps + group * g.M + row) : 0;
   };
 
@@ -301,17 +303,20 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
       // Every thread converts the pieces that it fetched.  (The multiplication
       // two stages ago, which read this buffer, has been waited for.)
 #pragma unroll
-      for (int j = 0; j < kZRows; ++j) {
-        const int r = warp + kOuterWarps * j;
-        const uint2 q = *(const uint2*)(st + z_to[j]);
-        const uint32_t step = __shfl_sync(~0u, steps, (lane >> 4) * kZRows + j);
-        uint32_t w[4];
+      for (int j = 0; j < FETCH; ++j) {
+        const int r = row0 + ROW_STEP * j;
+        const uint4 q = *(const uint4*)(st + z_to[j]);
+        const uint32_t step = __shfl_sync(~0u, steps, 4 * j + 2 * (lane >> 4) + (at_col >> 7));
+        uint32_t w[8];
         codes_to_16(BF16, q.x, step, w[0], w[1]);
         codes_to_16(BF16, q.y, step, w[2], w[3]);
-        const uint32_t at = z0 + (lane >> 3) * 8192 + r * 128 + (swz ^ ((uint32_t)(r & 7) << 4));
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
-                     "r"(w[2]), "r"(w[3])
-                     : "memory");
+        codes_to_16(BF16, q.z, step, w[4], w[5]);
+        codes_to_16(BF16, q.w, step, w[6], w[7]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(z0 + place(r, at_col + 8 * h)),
+                       "r"(w[4 * h]), "r"(w[4 * h + 1]), "r"(w[4 * h + 2]), "r"(w[4 * h + 3])
+                       : "memory");
       }
     }
     fence_proxy_async_smem();

@@ -130,6 +130,15 @@ __device__ __forceinline__ void ring_drain(uint64_t* full, int stages, int steps
 // ceil(r / 64) blocks of 64.
 __host__ __device__ inline int split_half(int r) { return r <= 32 ? 32 : (r + 63) / 64 * 64; }
 
+// Two FP32 values as high and low 16-bit parts, packed.
+__device__ __forceinline__ void split16(bool bf16, float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack16(bf16, a, b);
+  float ra = a - widen16(bf16, (uint16_t)hi), rb = b - widen16(bf16, (uint16_t)(hi >> 16));
+  if (!(fabsf(ra) <= 3.0e38f)) ra = 0.0f;  // not finite: the high part says so by itself
+  if (!(fabsf(rb) <= 3.0e38f)) rb = 0.0f;
+  lo = pack16(bf16, ra, rb);
+}
+
 // Rounds t to its high and low 16-bit parts and stores them in the split T.
 __device__ __forceinline__ void store_split(uint16_t* split, int64_t row, int half, int c, float t,
                                             bool bf16) {
