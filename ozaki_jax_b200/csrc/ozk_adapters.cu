@@ -706,7 +706,10 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   if (p.back && g.batch > 2) g.batch = 2;
   const size_t stage = (size_t)g.xrows * 128 + (size_t)g.batch * a_bytes;
   const size_t red = (size_t)kRows * (g.rp + 4) * 4;
-  const size_t room = (g.rp <= 64 ? 108 : 180) * 1024 - red;
+  // (Stages for one CTA per SM where there are no more: a stage takes its copy's
+  // latency divided by the stages in flight.)
+  const bool alone = g.rp > 64 || tiles * splits <= device_sm_count(dev);
+  const size_t room = (alone ? 180 : 108) * 1024 - red;
   g.stages = (int)(room / stage);
   if (g.stages > 8) g.stages = 8;
   size_t area = g.stages * stage + red;

@@ -87,12 +87,8 @@ __global__ void __launch_bounds__(kSortThreads)
     const uint32_t b = __ballot_sync(~0u, mine);
     if (lane == 0) s_warp[warp] = __popc(b);
     __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < kSortThreads / 32; ++w) {
-      const int c = s_warp[w];
-      before += w < warp ? c : 0;
-      all += c;
-    }
+    const int c = s_warp[lane];  // as many warps as lanes
+    const int before = __reduce_add_sync(~0u, lane < warp ? c : 0), all = __reduce_add_sync(~0u, c);
     if (mine) order[pos + before + __popc(b & ((1u << lane) - 1))] = (int32_t)(m0 + t);
     pos += all;
     __syncthreads();
