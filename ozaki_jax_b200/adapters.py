@@ -127,13 +127,13 @@ def adapters_grad(dY, X, W, A, B, ids, T, scale=1.0, input_grad=True):
     dX = torch.empty((M, K), dtype=dtype, device=dev) if input_grad else None
     dA, dB = torch.empty_like(A), torch.empty_like(B)
     lib = L.load()
-    y, w, a, b = dY.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr()
-    ready = not ((y | w | a | b) & 15 or (ldy | ldw | K | r) & 7)
+    x, y, w, a, b = Xd.data_ptr(), dY.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr()
+    ready = not ((x | y | w | a | b) & 15 or (ldx | ldy | ldw | K | r) & 7)
     with D.on_device(dev):
         n = lib.ozk_adapters_grad_workspace_bytes(M, N, K, r, E, ready)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         L.check(lib.ozk_adapters_grad(
-            y, ldy, Xd.data_ptr(), ldx, _ptr(exps), w, ldw, a, b, _ptr(ids), T.data_ptr(),
+            y, ldy, x, ldx, _ptr(exps), w, ldw, a, b, _ptr(ids), T.data_ptr(),
             _ptr(factors), alpha, _ptr(dX), K, dA.data_ptr(), dB.data_ptr(), M, N, K, r, E,
             DTYPES[dtype], ws.data_ptr(), n, D.status_word(dev), D.stream_handle(dev)))
     return dX, dA, dB

@@ -51,24 +51,6 @@ struct LinearArgs {
   uint64_t budget_ns;
 };
 
-// 8 or 16 consecutive output columns of one row.
-__device__ __forceinline__ void store_cols(void* Y, int64_t at, const uint32_t* v, int n, bool bf16,
-                                           bool vec) {
-  uint16_t* y = (uint16_t*)Y + at;
-  if (vec && n >= 8) {
-    uint4 q;
-    q.x = pack16(bf16, __uint_as_float(v[0]), __uint_as_float(v[1]));
-    q.y = pack16(bf16, __uint_as_float(v[2]), __uint_as_float(v[3]));
-    q.z = pack16(bf16, __uint_as_float(v[4]), __uint_as_float(v[5]));
-    q.w = pack16(bf16, __uint_as_float(v[6]), __uint_as_float(v[7]));
-    *(uint4*)y = q;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) y[i] = round16(bf16, __uint_as_float(v[i]));
-  }
-}
-
 // Sum over the CTAs of the cluster (at most 8), in rank order, of the four FP32
 // partials at shared-memory address `a` of each.  The loads are independent, so
 // their round trips overlap.
@@ -247,7 +229,8 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   tc_fence_after();
   const int mrows = g.M - row0 < kRows ? (int)(g.M - row0) : kRows;
-  if (splits == 1) {
+  if (splits == 1 && g.y_vec && col0 + BN <= g.N) {
+    // 16-byte stores of each row's columns.
     if (warp >= 2) {
       const int q = warp & 3;
       const int64_t row = row0 + q * 32 + lane;
@@ -256,16 +239,23 @@ __global__ void __launch_bounds__(kThreads)
         uint32_t v[32];
         tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c, v);
         tmem_wait_ld();
-        if (row < g.M)
+        if (row < g.M) {
+          uint4* y = (uint4*)((uint16_t*)g.Y + row * g.ldy + col0 + c);
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
-            const int n = g.N - (col0 + c + i);
-            if (n > 0) store_cols(g.Y, row * g.ldy + col0 + c + i, v + i, n, g.bf16, g.y_vec);
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              w[j] = pack16(g.bf16, __uint_as_float(v[i + 2 * j]), __uint_as_float(v[i + 2 * j + 1]));
+            y[i / 8] = make_uint4(w[0], w[1], w[2], w[3]);
           }
+        }
       }
     }
   } else {
-    // [row][BN + 4]: rows of 16-byte pieces, eight of them across all banks.
+    // Parts to be added up, or rows that take no vector stores: by way of shared
+    // memory, [row][BN + 4]: rows of 16-byte pieces, eight of them across all
+    // banks.
     constexpr int LDP = BN + 4;
     float* part = (float*)smem;
     if (warp >= 2) {
@@ -600,13 +590,27 @@ __global__ void __launch_bounds__(kLowThreads)
   }
 }
 
-__global__ void k_pad_rows(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd,
-                           int64_t rows, int64_t cols) {
-  const int64_t n = rows * ldd;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / ldd, c = i - r * ldd;
-    dst[i] = c < cols ? src[r * lds + c] : (uint16_t)0;
+// A thread copies 8 elements, read one by one (a warp reads 512 bytes side by
+// side) and written as 16 bytes; a CTA takes 256 columns of 32 rows.
+__global__ void __launch_bounds__(256)
+    k_pad_rows(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd, int64_t rows,
+               int64_t cols) {
+  const int64_t c = ((int64_t)blockIdx.x * 32 + threadIdx.x % 32) * 8;
+  if (c >= ldd) return;
+  for (int64_t r = (int64_t)blockIdx.y * 32 + threadIdx.x / 32; r < rows;
+       r += (int64_t)gridDim.y * 32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t row = r + 8 * j;
+      if (row >= rows) break;
+      const uint16_t* p = src + row * lds + c;
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = (c + 2 * i < cols ? p[2 * i] : 0u) |
+               ((c + 2 * i + 1 < cols ? (uint32_t)p[2 * i + 1] : 0u) << 16);
+      *(uint4*)(dst + row * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
@@ -615,10 +619,9 @@ __global__ void k_pad_rows(const uint16_t* src, int64_t lds, uint16_t* dst, int6
 int launch_pad_rows(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows,
                     int64_t cols, cudaStream_t stream) {
   if (rows == 0 || cols == 0) return OZK_OK;
-  int64_t blocks = (rows * ldd + 255) / 256;
-  if (blocks > 148 * 16) blocks = 148 * 16;
-  k_pad_rows<<<(unsigned)blocks, 256, 0, stream>>>((const uint16_t*)src, lds, (uint16_t*)dst, ldd,
-                                                   rows, cols);
+  const int64_t tiles = (rows + 31) / 32;
+  const dim3 grid((unsigned)((ldd + 255) / 256), (unsigned)(tiles < 65535 ? tiles : 65535));
+  k_pad_rows<<<grid, 256, 0, stream>>>((const uint16_t*)src, lds, (uint16_t*)dst, ldd, rows, cols);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? OZK_OK : set_cuda_error("k_pad_rows launch", e);
 }
@@ -681,8 +684,15 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   g.nkb = (int)((p.n_in + kKB - 1) / kKB);
   g.status = status;
   g.budget_ns = wait_budget_ns();
-  // Few rows (decoding): each may have an adapter of its own.
-  if (!p.back && p.M <= kRows) {
+  // Few rows (decoding): each may have an adapter of its own.  Up to 128 rows
+  // are taken one by one, up to 256 if that is cheaper than tiles in which
+  // every adapter has a row (about 1000 clocks for each batch's stage, against
+  // 2.5 KB of adapters read per clock).
+  const int accs = g.rp <= 64 ? 4 : 2;
+  const int64_t most = p.E < kRows ? p.E : kRows;
+  const int64_t by_tile = (most * accs * g.rp + 255) / 256 * (g.nkb / 8 + 1) * 1000;
+  const int64_t by_row = p.M * p.r * p.n_in * 2 / 2500;
+  if (!p.back && (p.M <= kRows || (p.M <= 2 * kRows && by_row < by_tile))) {
     const int half = split_half(p.r);
     k_low_rank_rows<<<dim3((unsigned)p.M, (unsigned)(half / kLowRanks)), kLowThreads, 0, stream>>>(
         (const uint16_t*)p.X.p, p.X.ld, (const uint16_t*)p.A.p, p.A.ld, p.n_in, g);
@@ -694,7 +704,6 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   // Two CTAs per SM at most (a second wave doubles the time), clusters of four
   // where there are tiles enough (of eight, only 15 fit the GPU at 100 KB of
   // shared memory a CTA), and chains of at most 512 elements.
-  const int accs = g.rp <= 64 ? 4 : 2;
   int splits = 1;
   while (splits < (tiles <= 8 ? 8 : 4) && tiles * splits * 2 <= 2 * device_sm_count(dev) &&
          g.nkb >= splits * 4)
@@ -747,7 +756,7 @@ int run_linear_bn(const Product& p, LinearArgs g, const uint16_t* split, int spl
   const size_t need = (size_t)(g.stages - 1) * g.xrows * 128 + kRows * 128;
   const size_t red = (size_t)g.xrows * (BN + 4) * 4;
   if (area < need) area = need;
-  if (splits > 1 && area < red) area = red;
+  if (area < red) area = red;
   if (area < tmem_share(BN)) area = tmem_share(BN);
   CUtensorMap mx, mw, mt, mb;
   int rc;
@@ -924,6 +933,7 @@ size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r,
   ws.take((size_t)N * round_up(K, 8) * 2);
   ws.take((size_t)E * r * round_up(K, 8) * 2);
   ws.take((size_t)E * N * round_up(r, 8) * 2);
+  ws.take((size_t)M * round_up(K, 8) * 2);
   return ws.used;
 }
 
@@ -956,14 +966,17 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   Arena ws(workspace);
   uint16_t* split = ws.take<uint16_t>((size_t)M * 4 * split_half(r));
   void* scratch = ws.take(outer_scratch_bytes(M, N, K, r, E, dev));
+  Operand in = {X, ldx};
   for (int pass = 0; pass < 2; ++pass) {
     Product q = p;
+    Operand x = in;
     Arena w = ws;
     if ((rc = align_operand(q.X, M, N, w, pass, s)) || (rc = align_operand(q.W, N, K, w, pass, s)) ||
         (rc = align_operand(q.A, (int64_t)E * N, r, w, pass, s)) ||
-        (rc = align_operand(q.B, (int64_t)E * r, K, w, pass, s)))
+        (rc = align_operand(q.B, (int64_t)E * r, K, w, pass, s)) ||
+        (!exps && (rc = align_operand(x, M, K, w, pass, s))))
       return rc;
-    if (pass) p = q;
+    if (pass) p = q, in = x;
     else if (!workspace || w.used > ws_bytes || ((uintptr_t)workspace & 127))
       return set_error(OZK_ERR_WORKSPACE, "workspace of %zu bytes, aligned to 128, needed", w.used);
   }
@@ -977,8 +990,8 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   o.r = r;
   o.E = E;
   o.ids = ids;
-  o.X = X;
-  o.ldx = ldx;
+  o.X = in.p;
+  o.ldx = in.ld;
   o.exps = (const int8_t*)exps;
   o.dY = p.X.p;
   o.ldy = p.X.ld;

@@ -11,7 +11,8 @@ struct OuterProduct {
   int64_t M, N, K;
   int r, E;
   const int32_t* ids;
-  const void* X;        // 16-bit [M][K], or int8 codes when exps is set
+  const void* X;        // 16-bit [M][K], or int8 codes when exps is set; X and dY on 16 bytes,
+                        // row strides too
   int64_t ldx;
   const int8_t* exps;
   const void* dY;       // [M][N]

@@ -102,7 +102,7 @@ struct OuterJob {
   const uint16_t* L;     // [M][2 split_half(r)]: high parts, low parts
   float* partial;        // [chunks + E][r C]
   void* out;             // [E][r][C], or [E][C][r] when trans
-  int trans, tiles, vec;
+  int trans, tiles;
 };
 
 struct OuterArgs {
@@ -226,7 +226,6 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
   const uint32_t z_bytes = left <= 0 ? 0 : CODES ? 16 : left < 8 ? 2 * (uint32_t)left : 16;
   const int64_t z_pitch = job.ldz * (CODES ? 1 : 2);
   const char* z_from = (const char*)job.Z + (z_bytes ? col * (CODES ? 1 : 2) : 0);
-  const bool vec = CODES || job.vec;
   // Where 8 columns of row r belong in the MMA's layout.
   auto place = [](int r, int c) {
     return (uint32_t)((c >> 6) * 8192 + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4));
@@ -245,18 +244,7 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
       const int row = rows[row0 + ROW_STEP * j];
       const char* p = z_from + (row >= 0 ? row : 0) * z_pitch;
       const uint32_t n = row >= 0 ? z_bytes : 0;
-      if (vec) {
-        cp_async16(zb + z_to[j], p, n);
-      } else {
-        const uint16_t* e = (const uint16_t*)p;
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = (4 * i < n ? e[2 * i] : 0u) | ((4 * i + 2 < n ? e[2 * i + 1] : 0u) << 16);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(zb + z_to[j]), "r"(w[0]),
-                     "r"(w[1]), "r"(w[2]), "r"(w[3])
-                     : "memory");
-      }
+      cp_async16(zb + z_to[j], p, n);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -366,15 +354,35 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
         tmem_ld16(at, v);
         tmem_ld16(at + g.rp, w);
         tmem_wait_ld();
-        if (c < job.C)
+        if (c >= job.C) continue;
+        float sum[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum[k] = __uint_as_float(v[k]) + __uint_as_float(w[k]);
+        if (job.trans && (g.r & 7) == 0) {
+          // a thread's ranks lie side by side: 8 at a time
+#pragma unroll
+          for (int k = 0; k < 16; k += 8) {
+            if (k0 + k >= g.r) break;
+            const int64_t to = c * g.r + k0 + k;
+            if (whole) {
+              *(uint4*)((uint16_t*)job.out + base + to) =
+                  make_uint4(pack16(BF16, sum[k], sum[k + 1]), pack16(BF16, sum[k + 2], sum[k + 3]),
+                             pack16(BF16, sum[k + 4], sum[k + 5]), pack16(BF16, sum[k + 6], sum[k + 7]));
+            } else {
+              float4* o = (float4*)(job.partial + part + to);
+              o[0] = make_float4(sum[k], sum[k + 1], sum[k + 2], sum[k + 3]);
+              o[1] = make_float4(sum[k + 4], sum[k + 5], sum[k + 6], sum[k + 7]);
+            }
+          }
+        } else {
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             if (k0 + k >= g.r) break;
-            const float sum = __uint_as_float(v[k]) + __uint_as_float(w[k]);
             const int64_t to = job.trans ? c * g.r + k0 + k : (int64_t)(k0 + k) * job.C + c;
-            if (whole) ((uint16_t*)job.out)[base + to] = round16(BF16, sum);
-            else job.partial[part + to] = sum;
+            if (whole) ((uint16_t*)job.out)[base + to] = round16(BF16, sum[k]);
+            else job.partial[part + to] = sum[k];
           }
+        }
       }
       tc_fence_before();
       __syncthreads();
@@ -441,12 +449,11 @@ __global__ void k_outer_join(const __grid_constant__ OuterArgs g) {
 }
 
 // Rows per chunk: the most chunks that run at once, one CTA per SM, each of at
-// least 256 rows (a second wave of a few CTAs would double the time).
+// least one stage (a second wave of a few CTAs would double the time).
 int chunk_len(int64_t M, int64_t tiles, int sms) {
   int64_t chunks = sms / tiles;
   if (chunks < 1) chunks = 1;
   int64_t len = round_up((M + chunks - 1) / chunks, kStep);
-  if (len < 256) len = 256;
   if (len > 8192) len = 8192;
   return (int)len;
 }
@@ -483,7 +490,6 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
   a.L = p.U;
   a.out = p.dA;
   a.tiles = (int)((p.K + kCols - 1) / kCols);
-  a.vec = ((uintptr_t)p.X & 15) == 0 && p.ldx % 8 == 0;
   OuterJob& b = g.job[1];
   b.Z = p.dY;
   b.ldz = p.ldy;
@@ -491,7 +497,6 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
   b.out = p.dB;
   b.trans = 1;
   b.tiles = (int)((p.N + kCols - 1) / kCols);
-  b.vec = ((uintptr_t)p.dY & 15) == 0 && p.ldy % 8 == 0;
   const int64_t tiles = a.tiles + b.tiles;
   g.len = chunk_len(p.M, tiles, device_sm_count(dev));
   const int64_t chunks = (p.M + g.len - 1) / g.len;

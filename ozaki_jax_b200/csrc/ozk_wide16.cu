@@ -47,6 +47,7 @@ constexpr int kABytes = kHalf * kKB * 2;
 constexpr int kRawBytes = kHalf * kKB;
 constexpr int kConvWarps = 4;    // of one of the two converter groups
 
+constexpr int kTurnBytes = 32 * 9 * 4;  // a warp's buffer for turning 8 columns of its 32 rows
 constexpr int kEpiWarps = 8;     // four lane quadrants, two column halves
 constexpr int kWork = 2 + kEpiWarps;  // first warp after the epilogue's
 
@@ -57,9 +58,10 @@ struct WideCfg {
   static constexpr int STAGES = SUB == 2 ? 4 : W ? 5 : 6;
   static constexpr int RAW = W ? (SUB == 2 ? 3 : 6) : 0;
   static constexpr int THREADS = 32 * (W ? kWork + 2 * kConvWarps + 1 : kWork + 1);
-  // All of an SM's shared memory: a CTA holds all TMEM columns, so no other
-  // TMEM kernel may share the SM.
-  static constexpr int SMEM = 227 * 1024 - (W ? 3 : SUB == 2 ? 20 : 11) * 1024;
+  // Most of an SM's shared memory, and in any case more than half: a CTA holds all
+  // TMEM columns, so no other TMEM kernel may fit beside it.
+  static constexpr int SMEM = 227 * 1024 - (W ? (SUB == 2 ? 1 : 3) : SUB == 2 ? 20 : 11) * 1024;
+  static_assert(1024 + STAGES * STAGE_BYTES + RAW * kRawBytes + kEpiWarps * kTurnBytes <= SMEM, "");
 };
 
 struct WideArgs {
@@ -90,37 +92,48 @@ __device__ __forceinline__ void tile_at(const WideArgs& g, int t, int& tm, int& 
   tn = r / rows;
 }
 
-// 32 consecutive outputs of one row, n of them inside the matrix, added to
-// what is there with `add`.
-__device__ __forceinline__ void store_f32(float* o, bool vec, int n, const uint32_t (&v)[32],
-                                          bool add) {
-  if (vec && n >= 32) {
+// 32 bytes at once (p on 32 bytes): a store of a warp touches 32 rows here, and
+// costs the same whether it writes a half or a whole sector of each.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// 32 consecutive outputs of one row, added to what is there with `add`.  wide:
+// the row takes 32-byte stores, else 16-byte ones.
+__device__ __forceinline__ void store_f32(float* o, bool wide, const uint32_t (&v)[32], bool add) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      float4 q = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]),
-                             __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-      if (add) {
-        const float4 p = *(const float4*)(o + i);
-        q.x += p.x, q.y += p.y, q.z += p.z, q.w += p.w;
-      }
-      *(float4*)(o + i) = q;
+  for (int i = 0; i < 32; i += 8) {
+    uint32_t f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = v[i + j];
+    if (add) {
+      const float4 p = *(const float4*)(o + i), q = *(const float4*)(o + i + 4);
+      const float w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = __float_as_uint(__uint_as_float(f[j]) + w[j]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) o[i] = __uint_as_float(v[i]) + (add ? o[i] : 0.0f);
+    if (wide) {
+      store32(o + i, f);
+    } else {
+      *(uint4*)(o + i) = make_uint4(f[0], f[1], f[2], f[3]);
+      *(uint4*)(o + i + 4) = make_uint4(f[4], f[5], f[6], f[7]);
+    }
   }
 }
-__device__ __forceinline__ void store_16(uint16_t* o, bool vec, int n, const uint32_t (&v)[32],
-                                         bool add, bool bf16) {
-  if (vec && n >= 32) {
+__device__ __forceinline__ void store_16(uint16_t* o, bool wide, const uint32_t (&v)[32], bool add,
+                                         bool bf16) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
+  for (int i = 0; i < 32; i += 16) {
+    uint32_t q[8];
+#pragma unroll
+    for (int h = 0; h < 16; h += 8) {
       float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[i + j]);
+      for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[i + h + j]);
       if (add) {
-        const uint4 p = *(const uint4*)(o + i);
+        const uint4 p = *(const uint4*)(o + i + h);
         const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -128,17 +141,40 @@ __device__ __forceinline__ void store_16(uint16_t* o, bool vec, int n, const uin
           f[2 * j + 1] += widen16(bf16, (uint16_t)(w[j] >> 16));
         }
       }
-      uint4 q;
-      q.x = pack16(bf16, f[0], f[1]);
-      q.y = pack16(bf16, f[2], f[3]);
-      q.z = pack16(bf16, f[4], f[5]);
-      q.w = pack16(bf16, f[6], f[7]);
-      *(uint4*)(o + i) = q;
-    }
-  } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) o[i] = round16(bf16, __uint_as_float(v[i]) + (add ? widen16(bf16, o[i]) : 0.0f));
+      for (int j = 0; j < 4; ++j) q[h / 2 + j] = pack16(bf16, f[2 * j], f[2 * j + 1]);
+    }
+    if (wide) {
+      store32(o + i, q);
+    } else {
+      *(uint4*)(o + i) = make_uint4(q[0], q[1], q[2], q[3]);
+      *(uint4*)(o + i + 8) = make_uint4(q[4], q[5], q[6], q[7]);
+    }
+  }
+}
+
+// The same for rows that take no vector stores, or the last n < 32 columns:
+// through the warp's own shared memory, so that a store writes along a row (a
+// lane storing its own row element by element touches 32 lines each time: a
+// 5905 x 7048 output took 447 us).  `out` is the warp's first row, `rows` of its
+// 32 lie inside the matrix.
+template <typename F>
+__device__ __forceinline__ void store_turned(uint8_t* turn, const uint32_t (&v)[32], int rows, int n,
+                                             F&& put) {
+  uint32_t* t = (uint32_t*)turn;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int h = 0; h < 32; h += 8) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[lane * 9 + i] = v[h + i];
+    __syncwarp();
+    const int c = h + (lane & 7);
+#pragma unroll
+    for (int r = 0; r < 32; r += 4) {
+      const int row = r + (lane >> 3);
+      if (row < rows && c < n) put(row, c, __uint_as_float(t[row * 9 + (lane & 7)]));
+    }
   }
 }
 
@@ -388,6 +424,7 @@ __global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
   } else if (warp < kWork) {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3, cbeg = (warp - 2) / 4 * (kTile / 2);
+    uint8_t* turn = sRaw + RAW * kRawBytes + (warp - 2) * kTurnBytes;
     int it = 0;
     bool ok = true;
     auto drain = [&](int buf, uint32_t parity, int64_t row0, int tn, int sp, bool add) {
@@ -407,15 +444,31 @@ __global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_u32(&acce[buf], 0));
         }
-        const int64_t left = g.N - (col0 + c);
-        if (row >= g.M || left <= 0) continue;
+        const int64_t left = g.N - (col0 + c), first = row - lane;
+        if (first >= g.M || left <= 0) continue;
         const int n = left < 32 ? (int)left : 32;
-        if (g.splits > 1)
-          store_f32(g.partial + ((int64_t)sp * g.M + row) * g.ldp + col0 + c, true, n, v, add);
-        else if (g.out_f32)
-          store_f32((float*)g.out + row * g.ldo + col0 + c, g.o_vec, n, v, add || g.accumulate);
-        else
-          store_16((uint16_t*)g.out + row * g.ldo + col0 + c, g.o_vec, n, v, g.accumulate, BF16);
+        if (g.splits > 1) {
+          if (row < g.M)  // (padded to whole pieces)
+            store_f32(g.partial + ((int64_t)sp * g.M + row) * g.ldp + col0 + c, true, v, add);
+        } else if (g.o_vec && n == 32) {
+          if (row >= g.M) continue;
+          if (g.out_f32)
+            store_f32((float*)g.out + row * g.ldo + col0 + c, g.o_vec > 1, v, add || g.accumulate);
+          else
+            store_16((uint16_t*)g.out + row * g.ldo + col0 + c, g.o_vec > 1, v, g.accumulate, BF16);
+        } else {
+          const int rows = g.M - first < 32 ? (int)(g.M - first) : 32;
+          const int64_t at = first * g.ldo + col0 + c;
+          store_turned(turn, v, rows, n, [&](int r, int i, float x) {
+            if (g.out_f32) {
+              float* o = (float*)g.out + at + r * g.ldo + i;
+              *o = x + (add || g.accumulate ? *o : 0.0f);
+            } else {
+              uint16_t* o = (uint16_t*)g.out + at + r * g.ldo + i;
+              *o = round16(BF16, x + (g.accumulate ? widen16(BF16, *o) : 0.0f));
+            }
+          });
+        }
       }
       return true;
     };
@@ -576,6 +629,12 @@ int wide_splits(int64_t M, int64_t N, int64_t C, int dev) {
   return s < 2 ? 1 : (int)s;
 }
 
+// Rows of the output take 32-byte (2), 16-byte (1) or no (0) vector stores.
+int wide_vec(const void* out, int64_t ldo, bool f32) {
+  const uintptr_t bits = (uintptr_t)out | (uintptr_t)(ldo * (f32 ? 4 : 2));
+  return bits % 32 == 0 ? 2 : bits % 16 == 0 ? 1 : 0;
+}
+
 template <WideMode MODE, int SUB>
 int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) {
   using Cfg = WideCfg<MODE, SUB>;
@@ -634,7 +693,7 @@ int launch_mode(const WideProduct& p, WideArgs g, int dev, cudaStream_t stream) 
 
 size_t wide_partial_bytes(int64_t M, int64_t N, int64_t C, int dev) {
   const int s = wide_splits(M, N, C, dev);
-  return s > 1 ? (size_t)s * M * round_up(N, 4) * 4 : 0;
+  return s > 1 ? (size_t)s * M * round_up(N, 32) * 4 : 0;
 }
 
 int launch_wide(const WideProduct& p, int dev, cudaStream_t stream) {
@@ -659,9 +718,9 @@ int launch_wide(const WideProduct& p, int dev, cudaStream_t stream) {
   g.accumulate = p.accumulate;
   g.out = p.out;
   g.ldo = p.ldo;
-  g.o_vec = ((uintptr_t)p.out & 15) == 0 && p.ldo % (p.out_f32 ? 4 : 8) == 0;
+  g.o_vec = wide_vec(p.out, p.ldo, p.out_f32);
   g.partial = p.partial;
-  g.ldp = round_up(p.N, 4);
+  g.ldp = round_up(p.N, 32);
   g.exps = p.exps;
   g.ids = p.ids;
   g.r = p.r;
