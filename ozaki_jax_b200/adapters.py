@@ -64,7 +64,8 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
     1 <= r <= 128.  Returns Y (M, N) in the type of X, or with return_low
     (Y, T), T (M, r) in float32, which adapters_grad takes.
 
-    Sums are FP32 and Y is rounded once.  T enters the second product as a sum
+    Like the other functions here it records nothing for autograd: the gradients
+    are adapters_grad's.  Sums are FP32 and Y is rounded once.  T enters the second product as a sum
     of two 16-bit values; in float16 |T| must stay below 65504.
     """
     (M, Kx), dtype = check_16bit("X", X)
@@ -77,7 +78,7 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
     ids = None if ids is None else ids.contiguous()
     Y = torch.empty((M, N), dtype=dtype, device=dev)
     low = torch.empty((M, r), dtype=torch.float32, device=dev) if return_low else None
-    if M and N:
+    if M and (N or return_low):
         lib = L.load()
         x, w, a, b = X.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr()
         ready = not ((x | w | a | b) & 15 or (ldx | ldw | K | r) & 7)
@@ -88,8 +89,6 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
                 x, ldx, w, ldw, a, b, _ptr(ids), _ptr(factors), alpha, Y.data_ptr(), N, _ptr(low),
                 M, N, K, r, E, DTYPES[dtype], ws.data_ptr(), n, D.status_word(dev),
                 D.stream_handle(dev)))
-    elif low is not None:
-        low.zero_()
     return (Y, low) if return_low else Y
 
 

@@ -877,7 +877,7 @@ extern "C" {
 
 size_t ozk_matmul_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E,
                                            int aligned) {
-  if (M < 1 || N < 1 || K < 1 || r < 1 || r > kMaxRank || E < 1) return 0;
+  if (M < 1 || N < 0 || K < 1 || r < 1 || r > kMaxRank || E < 1) return 0;
   Arena ws(nullptr);
   ws.take<uint16_t>((size_t)M * 4 * split_half(r));
   if (aligned) return ws.used;
@@ -896,9 +896,9 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
                         void* stream) {
   int rc = adapter_args(X, ldx, W, ldw, A, B, M, N, K, r, E, dt);
   if (rc) return rc;
-  if (M == 0 || N == 0) return OZK_OK;
-  if (ldx < K) return set_error(OZK_ERR_ARG, "ldx < K");
-  if (!Y || ldy < N) return set_error(OZK_ERR_ARG, "NULL Y or ldy < N");
+  if (M == 0 || (N == 0 && !low)) return OZK_OK;
+  if (ldx < K || !X || !A) return set_error(OZK_ERR_ARG, "NULL X or A, or ldx < K");
+  if (N && (!Y || ldy < N)) return set_error(OZK_ERR_ARG, "NULL Y or ldy < N");
   cudaStream_t s = (cudaStream_t)stream;
   int dev;
   cudaGetDevice(&dev);
@@ -908,15 +908,17 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
   for (int pass = 0; pass < 2; ++pass) {  // count first, then copy
     Product q = p;
     Arena w = ws;
-    if ((rc = align_operand(q.X, M, K, w, pass, s)) || (rc = align_operand(q.W, N, K, w, pass, s)) ||
+    if ((rc = align_operand(q.X, M, K, w, pass, s)) ||
         (rc = align_operand(q.A, (int64_t)E * r, K, w, pass, s)) ||
-        (rc = align_operand(q.B, (int64_t)E * N, r, w, pass, s)))
+        (N && (rc = align_operand(q.W, N, K, w, pass, s))) ||
+        (N && (rc = align_operand(q.B, (int64_t)E * N, r, w, pass, s))))
       return rc;
     if (pass) p = q;
     else if (!workspace || w.used > ws_bytes || ((uintptr_t)workspace & 127))
       return set_error(OZK_ERR_WORKSPACE, "workspace of %zu bytes, aligned to 128, needed", w.used);
   }
-  if ((rc = run_low_rank(p, ids, scale, (float)alpha, low, split, status_dev, dev, s))) return rc;
+  if ((rc = run_low_rank(p, ids, scale, (float)alpha, low, split, status_dev, dev, s)) || N == 0)
+    return rc;
   return run_linear(p, ids, split, Y, ldy, status_dev, dev, s);
 }
 

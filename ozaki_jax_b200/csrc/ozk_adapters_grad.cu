@@ -100,10 +100,14 @@ struct OuterJob {
   int64_t ldz, C;
   const int8_t* exps;    // [groups][M]
   const uint16_t* L;     // [M][2 split_half(r)]: high parts, low parts
-  float* partial;        // [chunks + E][r C]
+  float* partial;        // [2 chunks][r C], see below
   void* out;             // [E][r][C], or [E][C][r] when trans
   int trans, tiles;
 };
+
+// Of the adapters in a chunk, only the first (continued from the chunk before)
+// and the last (continued in the next) can have rows elsewhere: two places of
+// partial sums per chunk, the second for an adapter that does not start it.
 
 struct OuterArgs {
   OuterJob job[2];
@@ -346,7 +350,7 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
       const bool whole = was.first == __ldg(g.start + was.e) && was.end == __ldg(g.start + was.e + 1);
       const int mb = (warp >> 2) & 1, q = warp & 3;
       const int64_t c = col0 + mb * 128 + q * 32 + lane;
-      const int64_t part = (int64_t)(chunk + was.e) * g.r * job.C;
+      const int64_t part = (int64_t)(2 * chunk + (was.first != chunk * g.len)) * g.r * job.C;
       const int64_t base = (int64_t)was.e * g.r * job.C;
       for (int k0 = (warp >> 3) * 16; fetcher && k0 < g.rp; k0 += 32) {  // two warps share a quadrant
         uint32_t v[16], w[16];
@@ -443,7 +447,8 @@ __global__ void k_outer_join(const __grid_constant__ OuterArgs g) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
        i += (int64_t)gridDim.x * blockDim.x) {
     float s = 0.0f;
-    for (int c = c0; c <= c1; ++c) s += job.partial[(int64_t)(c + e) * n + i];
+    for (int c = c0; c <= c1; ++c)
+      s += job.partial[(int64_t)(2 * c + (c == c0 && a != c0 * g.len)) * n + i];
     ((uint16_t*)job.out)[e * n + i] = round16(g.bf16, s);
   }
 }
@@ -468,8 +473,8 @@ size_t outer_scratch_bytes(int64_t M, int64_t N, int64_t K, int r, int E, int de
   ws.take((size_t)M * 4);
   ws.take((size_t)(E + 1) * 4);
   ws.take((size_t)M * 4 * split_half(r));
-  ws.take((size_t)(chunks + E) * r * K * 4);
-  ws.take((size_t)(chunks + E) * r * N * 4);
+  ws.take((size_t)2 * chunks * r * K * 4);
+  ws.take((size_t)2 * chunks * r * N * 4);
   return ws.used;
 }
 
@@ -506,8 +511,8 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
   int32_t* start = ws.take<int32_t>((size_t)(p.E + 1) * 4);
   uint16_t* split = ws.take<uint16_t>((size_t)p.M * 4 * split_half(p.r));
   b.L = split;
-  a.partial = ws.take<float>((size_t)(chunks + p.E) * p.r * p.K * 4);
-  b.partial = ws.take<float>((size_t)(chunks + p.E) * p.r * p.N * 4);
+  a.partial = ws.take<float>((size_t)2 * chunks * p.r * p.K * 4);
+  b.partial = ws.take<float>((size_t)2 * chunks * p.r * p.N * 4);
   g.order = order;
   g.start = start;
   int64_t more = (p.M * split_half(p.r) + 4 * kSortThreads - 1) / (4 * kSortThreads);

@@ -208,8 +208,9 @@ def test_empty():
     X, W, A, B, ids, scale, dY = make(4, 16, 32, 4, 2, F16)
     Y, T = oz.matmul_adapters(X[:0], W, A, B, ids[:0], scale, return_low=True)
     assert Y.shape == (0, 16) and T.shape == (0, 4)
-    Y = oz.matmul_adapters(X, W[:0], A, B[:, :0], ids, scale)
-    assert Y.shape == (4, 0)
+    Y, wide = oz.matmul_adapters(X, W[:0], A, B[:, :0], ids, scale, return_low=True)
+    assert Y.shape == (4, 0)  # T does not depend on the projection's width
+    assert torch.equal(wide, oz.matmul_adapters(X, W, A, B, ids, scale, return_low=True)[1])
     dX, dA, dB = oz.adapters_grad(dY[:0], X[:0], W, A, B, ids[:0], T, scale)
     assert dX.shape == (0, 32) and bool((dA == 0).all()) and bool((dB == 0).all())
     dX, dA, dB = oz.adapters_grad(dY[:, :0], X, W[:0], A, B[:, :0], ids, torch.ones(4, 4).cuda(), scale)
@@ -239,6 +240,51 @@ def test_strides_and_alignment():
             assert all(torch.equal(a, b) for a, b in zip(got, grads))
         every = torch.stack([ids, ids], 1)
         assert torch.equal(oz.matmul_adapters(X, W, A, B, every[:, 0], scale), want)
+
+
+def test_many_adapters_over_chunks():
+    """More adapters than rows in a chunk, adapters over several chunks, adapters without rows;
+    single-row requests in the forward pass."""
+    M, N, K, r, E = 3000, 72, 600, 8, 700
+    X, W, A, B, ids, scale, dY = make(M, N, K, r, E, BF16, seed=4)
+    ids[:900] = 650
+    ids[900:1000] = 3
+    T = torch.randn(M, r, device="cuda")
+    got = oz.adapters_grad(dY, X, W, A, B, ids, T, scale)
+    want, size = grads64(dY, X, W, A, B, ids, T, scale)
+    u = torch.finfo(BF16).eps / 2
+    for g, w, m, n in zip(got, want, size, (N + 2 * r + 4, M + N + 4, M + 4)):
+        check(g, w, m, n, u)
+    Y = oz.matmul_adapters(X, W, A, B, ids, scale)
+    want, _, mY, _ = forward64(X, W, A, B, ids, scale)
+    check(Y, want, mY, K + 2 * r + 4, u)
+
+
+def test_first_call_of_a_process_may_be_captured():
+    """Kernels are loaded and the status word is made inside the capture."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    code = (
+        "import torch, ozaki_jax_b200 as oz\n"
+        "r = lambda *s: torch.randn(*s, device='cuda').bfloat16()\n"
+        "X, W, A, B, dY = r(40, 64), r(48, 64), r(2, 8, 64), r(2, 48, 8), r(40, 48)\n"
+        "ids = torch.randint(0, 2, (40,), device='cuda', dtype=torch.int32)\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "def step():\n"
+        "    s = oz.checkpoint_rows(X)\n"
+        "    Y, T = oz.matmul_adapters(X, W, A, B, ids, 0.5, return_low=True)\n"
+        "    return (Y, T, *oz.adapters_grad(dY, s, W, A, B, ids, T, 0.5),\n"
+        "            oz.checkpoint_grad(dY, s), oz.restore_rows(s))\n"
+        "with torch.cuda.graph(g):\n"
+        "    out = step()\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "assert all(torch.equal(a, b) for a, b in zip(out, step()))\n"
+        "print('captured')\n")
+    p = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True,
+                       timeout=120)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stderr[-2000:]
 
 
 def test_streams_and_graphs():
