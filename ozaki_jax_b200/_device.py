@@ -122,8 +122,11 @@ class _Here:
 _HERE = _Here()
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def on_device(device):
-    """Context in which `device` is the current CUDA device."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    """Context in which `device`, that of a CUDA tensor, is the current one."""
+    if device.index == _current_device():
         return _HERE
     return torch.cuda.device(device)

@@ -76,14 +76,14 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
     (X, ldx), (W, ldw) = row_major(X), row_major(W)
     A, B = A.contiguous(), B.contiguous()
     ids = None if ids is None else ids.contiguous()
-    Y = torch.empty((M, N), dtype=dtype, device=dev)
-    low = torch.empty((M, r), dtype=torch.float32, device=dev) if return_low else None
+    Y = X.new_empty((M, N))
+    low = X.new_empty((M, r), dtype=torch.float32) if return_low else None
     if M and (N or return_low):
         lib = L.load()
         x, w, a, b = X.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr()
         ready = not ((x | w | a | b) & 15 or (ldx | ldw | K | r) & 7)
         n = lib.ozk_matmul_adapters_workspace_bytes(M, N, K, r, E, ready)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        ws = X.new_empty(n, dtype=torch.uint8)
         with D.on_device(dev):
             L.check(lib.ozk_matmul_adapters(
                 x, ldx, w, ldw, a, b, _ptr(ids), _ptr(factors), alpha, Y.data_ptr(), N, _ptr(low),
@@ -123,14 +123,14 @@ def adapters_grad(dY, X, W, A, B, ids, T, scale=1.0, input_grad=True):
     (dY, ldy), (W, ldw) = row_major(dY), row_major(W)
     A, B, T = A.contiguous(), B.contiguous(), T.contiguous()
     ids = None if ids is None else ids.contiguous()
-    dX = torch.empty((M, K), dtype=dtype, device=dev) if input_grad else None
+    dX = dY.new_empty((M, K)) if input_grad else None
     dA, dB = torch.empty_like(A), torch.empty_like(B)
     lib = L.load()
     x, y, w, a, b = Xd.data_ptr(), dY.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr()
     ready = not ((x | y | w | a | b) & 15 or (ldx | ldy | ldw | K | r) & 7)
     with D.on_device(dev):
         n = lib.ozk_adapters_grad_workspace_bytes(M, N, K, r, E, ready)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        ws = dY.new_empty(n, dtype=torch.uint8)
         L.check(lib.ozk_adapters_grad(
             y, ldy, x, ldx, _ptr(exps), w, ldw, a, b, _ptr(ids), T.data_ptr(),
             _ptr(factors), alpha, _ptr(dX), K, dA.data_ptr(), dB.data_ptr(), M, N, K, r, E,

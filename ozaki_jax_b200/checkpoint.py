@@ -76,13 +76,15 @@ def checkpoint_rows(X):
     dev = check_device(X)
     X, ldx = row_major(X)
     groups = (K + GROUP - 1) // GROUP
-    codes = torch.empty((M, groups * GROUP), dtype=torch.int8, device=dev)
-    exps = torch.empty((groups, M), dtype=torch.int8, device=dev)
+    codes = X.new_empty((M, groups * GROUP), dtype=torch.int8)
+    exps = codes.new_empty((groups, M))
     with D.on_device(dev):
         L.check(L.load().ozk_checkpoint_rows(X.data_ptr(), ldx, M, K, DTYPES[dtype],
                                              codes.data_ptr(), groups * GROUP, exps.data_ptr(),
                                              D.stream_handle(dev)))
-    return SavedRows(codes, exps, K, dtype)
+    saved = object.__new__(SavedRows)  # as __init__ would leave it, its checks apart
+    saved.codes, saved.exps, saved.cols, saved.dtype = codes, exps, K, dtype
+    return saved
 
 
 def restore_rows(saved, dtype=None):
@@ -93,11 +95,12 @@ def restore_rows(saved, dtype=None):
     if dtype not in (saved.dtype, torch.float32):
         raise ValueError(f"dtype={dtype}; expected {saved.dtype} or float32.")
     dev = check_device(saved.codes)
-    M, K = saved.shape
-    out = torch.empty((M, K), dtype=dtype, device=dev)
+    codes, K = saved.codes, saved.cols
+    M, ldc = codes.shape
+    out = codes.new_empty((M, K), dtype=dtype)
     with D.on_device(dev):
-        L.check(L.load().ozk_restore_rows(saved.codes.data_ptr(), saved.codes.shape[1],
-                                          saved.exps.data_ptr(), M, K, out.data_ptr(), K,
+        L.check(L.load().ozk_restore_rows(codes.data_ptr(), ldc, saved.exps.data_ptr(), M, K,
+                                          out.data_ptr(), K,
                                           DTYPES[dtype], D.stream_handle(dev)))
     return out
 
@@ -126,7 +129,7 @@ def checkpoint_grad(dY, saved, out=None, accumulate=False, dtype=None):
         dtype = dtype_y if dtype is None else dtype
         if dtype not in (dtype_y, torch.float32):
             raise ValueError(f"dtype={dtype}; expected {dtype_y} or float32.")
-        out = torch.empty((N, K), dtype=dtype, device=dev)
+        out = dY.new_empty((N, K), dtype=dtype)
     else:
         check_matrix("out", out, rows=N, cols=K)
         if out.dtype not in (dtype_y, torch.float32):
@@ -140,7 +143,7 @@ def checkpoint_grad(dY, saved, out=None, accumulate=False, dtype=None):
     y = dY.data_ptr()
     with D.on_device(dev):
         n = lib.ozk_checkpoint_grad_workspace_bytes(M, N, K, not (y & 15 or ldy & 7))
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        ws = saved.codes.new_empty(n)
         L.check(lib.ozk_checkpoint_grad(
             y, ldy, saved.codes.data_ptr(), saved.codes.shape[1],
             saved.exps.data_ptr(), out.data_ptr(), out.stride(0) if N > 1 else K, M, N, K,

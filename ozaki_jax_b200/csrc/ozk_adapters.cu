@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(kThreads)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_release();
   const uint32_t tmem = s_tmem;
 
   if (warp == 0) {
@@ -481,6 +482,9 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   cluster_sync();
+  // The kernel before this one may still run (the backward pass's row lists):
+  // whoever waits for this kernel has waited for that one too.
+  if (threadIdx.x == 0) grid_wait();
   // Rows of the tile are dealt to the CTAs of the cluster.
   const int mrows = g.M - row0 < kRows ? (int)(g.M - row0) : kRows;
   const int half = split_half(g.r);
@@ -738,7 +742,7 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
     rc = make_map(&ma, p.A.p, 2, p.n_in, p.r, p.E, p.A.ld * 2, p.A.ld * 2 * p.r, kKB, g.rp, true);
   if (rc) return rc;
   return p.back ? launch_cluster<k_low_rank<true>>("k_low_rank", tiles, splits, kThreads,
-                                                   area + 1024, false, dev, stream, mx, ma, g)
+                                                   area + 1024, true, dev, stream, mx, ma, g)
                 : launch_cluster<k_low_rank<false>>("k_low_rank", tiles, splits, kThreads,
                                                     area + 1024, false, dev, stream, mx, ma, g);
 }
@@ -982,8 +986,6 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
     else if (!workspace || w.used > ws_bytes || ((uintptr_t)workspace & 127))
       return set_error(OZK_ERR_WORKSPACE, "workspace of %zu bytes, aligned to 128, needed", w.used);
   }
-  if ((rc = run_low_rank(p, ids, scale, (float)alpha, nullptr, split, status_dev, dev, s))) return rc;
-  if (dX && (rc = run_linear(p, ids, split, dX, lddx, status_dev, dev, s))) return rc;
   OuterProduct o = {};
   o.bf16 = p.bf16;
   o.M = M;
@@ -1002,6 +1004,9 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   o.dA = dA;
   o.dB = dB;
   o.status = status_dev;
+  if ((rc = launch_outer_rows(o, scratch, dev, s))) return rc;
+  if ((rc = run_low_rank(p, ids, scale, (float)alpha, nullptr, split, status_dev, dev, s))) return rc;
+  if (dX && (rc = run_linear(p, ids, split, dX, lddx, status_dev, dev, s))) return rc;
   return launch_outer(o, scratch, dev, s);
 }
 

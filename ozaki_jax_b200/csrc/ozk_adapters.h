@@ -24,6 +24,10 @@ struct OuterProduct {
 };
 
 size_t outer_scratch_bytes(int64_t M, int64_t N, int64_t K, int r, int E, int dev);
+// First the row lists and T's split (the kernel that follows may start early and
+// must wait for them before it ends), then, after the kernel that makes U, the
+// sums.
+int launch_outer_rows(const OuterProduct& p, void* scratch, int dev, cudaStream_t stream);
 int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t stream);
 
 }  // namespace ozk

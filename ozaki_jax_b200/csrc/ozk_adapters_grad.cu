@@ -45,6 +45,7 @@ constexpr int kZBytes = kCols * kStep * 2;
 __global__ void __launch_bounds__(kSortThreads)
     k_sort_rows(const int32_t* ids, int64_t M, int E, int32_t* order, int32_t* start,
                 const float* T, int r, uint16_t* split, int bf16) {
+  grid_release();
   if ((int)blockIdx.x >= E) {  // the CTAs after the adapters': the split of T
     const int half = split_half(r);
     const int64_t n = M * half;
@@ -407,6 +408,8 @@ __global__ void __launch_bounds__(kOuterThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ OuterShared sh;
+  grid_release();
+  grid_wait();  // for U, by way of the kernels between them for the row lists
   const bool second = (int)blockIdx.x >= g.job[0].tiles;
   const OuterJob& job = g.job[second];
   const int64_t col0 = (int64_t)((int)blockIdx.x - (second ? g.job[0].tiles : 0)) * kCols;
@@ -438,6 +441,7 @@ __global__ void __launch_bounds__(kOuterThreads, 1)
 
 // Adapters whose rows lie in several chunks (or that have none).
 __global__ void k_outer_join(const __grid_constant__ OuterArgs g) {
+  grid_wait();
   const int e = blockIdx.y;
   const OuterJob& job = g.job[blockIdx.z];
   const int a = __ldg(g.start + e), b = __ldg(g.start + e + 1);
@@ -465,20 +469,72 @@ int chunk_len(int64_t M, int64_t tiles, int sms) {
 
 }  // namespace
 
+namespace {
+
+// The scratch of one call.
+struct OuterScratch {
+  int32_t *order, *start;
+  uint16_t* split;  // of T
+  float *pa, *pb;
+  int len;
+  int64_t chunks, tiles;
+};
+
+OuterScratch outer_scratch(int64_t M, int64_t N, int64_t K, int r, int E, int dev, Arena& ws) {
+  OuterScratch s;
+  s.tiles = (N + kCols - 1) / kCols + (K + kCols - 1) / kCols;
+  s.len = chunk_len(M, s.tiles, device_sm_count(dev));
+  s.chunks = (M + s.len - 1) / s.len;
+  s.order = ws.take<int32_t>((size_t)M * 4);
+  s.start = ws.take<int32_t>((size_t)(E + 1) * 4);
+  s.split = ws.take<uint16_t>((size_t)M * 4 * split_half(r));
+  s.pa = ws.take<float>((size_t)2 * s.chunks * r * K * 4);
+  s.pb = ws.take<float>((size_t)2 * s.chunks * r * N * 4);
+  return s;
+}
+
+// A launch that may begin while the kernel before it, which has released it,
+// still runs; the kernel waits for that one itself.
+template <typename K>
+int launch_early(const char* what, K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                 const OuterArgs& g) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, g);
+  return e == cudaSuccess ? OZK_OK : set_cuda_error(what, e);
+}
+
+}  // namespace
+
 size_t outer_scratch_bytes(int64_t M, int64_t N, int64_t K, int r, int E, int dev) {
-  const int64_t tiles = (N + kCols - 1) / kCols + (K + kCols - 1) / kCols;
-  const int64_t chunks = (M + chunk_len(M, tiles, device_sm_count(dev)) - 1) /
-                         chunk_len(M, tiles, device_sm_count(dev));
   Arena ws(nullptr);
-  ws.take((size_t)M * 4);
-  ws.take((size_t)(E + 1) * 4);
-  ws.take((size_t)M * 4 * split_half(r));
-  ws.take((size_t)2 * chunks * r * K * 4);
-  ws.take((size_t)2 * chunks * r * N * 4);
+  outer_scratch(M, N, K, r, E, dev, ws);
   return ws.used;
 }
 
+int launch_outer_rows(const OuterProduct& p, void* scratch, int dev, cudaStream_t stream) {
+  Arena ws(scratch);
+  const OuterScratch o = outer_scratch(p.M, p.N, p.K, p.r, p.E, dev, ws);
+  int64_t more = (p.M * split_half(p.r) + 4 * kSortThreads - 1) / (4 * kSortThreads);
+  if (more > 148) more = 148;
+  k_sort_rows<<<(unsigned)(p.E + more), kSortThreads, 0, stream>>>(
+      p.ids, p.M, p.E, o.order, o.start, p.T, p.r, o.split, p.bf16);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? OZK_OK : set_cuda_error("k_sort_rows launch", e);
+}
+
 int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t stream) {
+  Arena ws(scratch);
+  const OuterScratch sc = outer_scratch(p.M, p.N, p.K, p.r, p.E, dev, ws);
+  if (sc.chunks > 65535) return set_error(OZK_ERR_UNSUPPORTED, "too many rows");
   OuterArgs g = {};
   g.M = p.M;
   g.E = p.E;
@@ -487,40 +543,27 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
   g.bf16 = p.bf16;
   g.status = p.status;
   g.budget_ns = wait_budget_ns();
+  g.order = sc.order;
+  g.start = sc.start;
+  g.len = sc.len;
   OuterJob& a = g.job[0];
   a.Z = p.X;
   a.ldz = p.ldx;
   a.C = p.K;
   a.exps = p.exps;
   a.L = p.U;
+  a.partial = sc.pa;
   a.out = p.dA;
   a.tiles = (int)((p.K + kCols - 1) / kCols);
   OuterJob& b = g.job[1];
   b.Z = p.dY;
   b.ldz = p.ldy;
   b.C = p.N;
+  b.L = sc.split;
+  b.partial = sc.pb;
   b.out = p.dB;
   b.trans = 1;
   b.tiles = (int)((p.N + kCols - 1) / kCols);
-  const int64_t tiles = a.tiles + b.tiles;
-  g.len = chunk_len(p.M, tiles, device_sm_count(dev));
-  const int64_t chunks = (p.M + g.len - 1) / g.len;
-  if (chunks > 65535) return set_error(OZK_ERR_UNSUPPORTED, "too many rows");
-  Arena ws(scratch);
-  int32_t* order = ws.take<int32_t>((size_t)p.M * 4);
-  int32_t* start = ws.take<int32_t>((size_t)(p.E + 1) * 4);
-  uint16_t* split = ws.take<uint16_t>((size_t)p.M * 4 * split_half(p.r));
-  b.L = split;
-  a.partial = ws.take<float>((size_t)2 * chunks * p.r * p.K * 4);
-  b.partial = ws.take<float>((size_t)2 * chunks * p.r * p.N * 4);
-  g.order = order;
-  g.start = start;
-  int64_t more = (p.M * split_half(p.r) + 4 * kSortThreads - 1) / (4 * kSortThreads);
-  if (more > 148) more = 148;
-  k_sort_rows<<<(unsigned)(p.E + more), kSortThreads, 0, stream>>>(p.ids, p.M, p.E, order, start,
-                                                                   p.T, p.r, split, p.bf16);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return set_cuda_error("k_sort_rows launch", e);
   // One CTA per SM: as many stages, up to four, as fit.
   const int l_bytes = (2 * g.rp + 63) / 64 * 8192;
   const int stages = l_bytes > 16384 ? 3 : 4;
@@ -536,15 +579,14 @@ int launch_outer(const OuterProduct& p, void* scratch, int dev, cudaStream_t str
                   : (stages == 4 ? allow_smem<k_outer<false, 4>>(smem, dev)
                                  : allow_smem<k_outer<false, 3>>(smem, dev));
   if (rc) return rc;
-  kern<<<dim3((unsigned)tiles, (unsigned)chunks), kOuterThreads, smem, stream>>>(g);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return set_cuda_error("k_outer launch", e);
+  rc = launch_early("k_outer launch", kern, dim3((unsigned)sc.tiles, (unsigned)sc.chunks),
+                    kOuterThreads, smem, stream, g);
+  if (rc) return rc;
   const int64_t most = (int64_t)p.r * (p.K > p.N ? p.K : p.N);
   int64_t blocks = (most + 1023) / 1024;
   if (blocks > 256) blocks = 256;
-  k_outer_join<<<dim3((unsigned)blocks, (unsigned)p.E, 2), 256, 0, stream>>>(g);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? OZK_OK : set_cuda_error("k_outer_join launch", e);
+  return launch_early("k_outer_join launch", k_outer_join,
+                      dim3((unsigned)blocks, (unsigned)p.E, 2), 256, 0, stream, g);
 }
 
 }  // namespace ozk

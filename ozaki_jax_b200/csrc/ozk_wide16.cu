@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
   __syncthreads();
   cluster_sync();
   tc_fence_after();
+  grid_release();
   const uint32_t tmem = s_tmem;
 
   auto item_at = [&](int i, int& tm, int& tn, int& sp, int& kb0, int& kb1) {
