@@ -76,6 +76,11 @@ __device__ __forceinline__ float4 cluster_sum4(uint32_t a, int splits) {
 
 // ---------------------------------------------------------------- k_linear
 //
+// Few rows: bound by reading W once (one row of 4096 x 4096: the call takes 11 us
+// in a graph, of which W's 33.5 MB need 5.1; 64 rows of 8192 x 4096 with 64
+// adapters: 20 us, 12.9 by their bytes).  The tokens are the MMA's M side even
+// then: 128 lanes of which few are used cost N / 2 clocks per 16 indexes, less
+// than the 1.4 N that W's bytes take from memory.
 // One CTA per 128 x BN tile, or a cluster of CTAs per tile that split the
 // contraction (and the adapters) between them and add their FP32 partials in
 // rank order through distributed shared memory: deterministic, no scratch.

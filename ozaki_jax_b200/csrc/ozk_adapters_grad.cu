@@ -17,6 +17,9 @@
 // rows up, beside the sixteen that fetch: with the issue and the lookup in the
 // fetching warps a stage took 5400 clocks.  Rows of other
 // adapters are never read, so a NaN in them cannot reach this one's gradient.
+// 4096 rows, N = K = 4096, r = 16: 34 us; 8192 rows, N = 4096, K = 8192 as codes,
+// r = 32: 96 us, a stage of 64 rows taking about 3700 clocks, most of it the
+// fetching warps' own chain of copies, conversion and barriers.
 // A chunk that holds all of an adapter's rows writes its gradient at once;
 // otherwise the chunks' FP32 sums are added in order by k_outer_join: the
 // result does not depend on scheduling.

@@ -17,7 +17,10 @@
 //
 // Both kernels are bound by HBM: one read and one write of each element.  A
 // CTA takes 32 rows x 256 columns, a warp 4 rows, each lane 16 bytes of each
-// (four loads in flight).
+// (four loads in flight).  65536 x 4096 BF16: saved in 134 us (6.0 TB/s), restored
+// in 121 us (6.6 TB/s); a plain copy of the matrix runs at 6.4 TB/s.  With the
+// maxima and codes computed element by element in FP32 (17 instructions an
+// element instead of 11) saving was bound by instructions: 220 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
