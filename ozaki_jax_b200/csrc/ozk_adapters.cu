@@ -22,7 +22,6 @@
 // the price of r more columns of the contraction.
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -92,7 +91,7 @@ __global__ void __launch_bounds__(kThreads)
              const __grid_constant__ CUtensorMap mapT, const __grid_constant__ CUtensorMap mapB,
              const __grid_constant__ LinearArgs g) {
   constexpr int B_BYTES = BN * 128;
-  constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+  constexpr int TMEM_COLS = BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int a_bytes = g.xrows * 128;
@@ -224,8 +223,7 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
   } else {
     if (warp == 2) {
-      if (g.r > 0) build_slots<4>(g.ids, row0, g.M, g.E, &slots, lane);
-      else if (lane == 0) slots.n = 0;
+      build_slots<4>(g.ids, row0, g.M, g.E, &slots, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(&slots_ready);
     }

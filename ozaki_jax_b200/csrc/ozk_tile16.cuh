@@ -87,18 +87,32 @@ __device__ __forceinline__ float widen16(bool bf16, uint16_t u) {
   return bf16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
 }
 
-// mbar_wait that also acquires what a peer CTA's threads wrote before their
-// (cluster-scope) arrivals.
+// mbar_wait that acquires at cluster scope: what a peer CTA's threads wrote
+// before their arrivals (mbar_arrive_cluster).
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
                                                   volatile int* abort, int32_t* status,
                                                   uint64_t budget_ns) {
-  if (!mbar_wait(bar, parity, abort, status, budget_ns)) return false;
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-  return true;
-}
-
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (i == 1) t0 = global_ns();
+    if ((i & 63) == 0) {
+      if (abort && *abort) return false;
+      if (global_ns() - t0 > budget_ns) {
+        if (abort) *abort = 1;
+        raise_flag(status, OZK_FLAG_TIMEOUT);
+        return false;
+      }
+    }
+  }
 }
 
 // Ring of shared-memory stages: the index and phase parity of the current step.

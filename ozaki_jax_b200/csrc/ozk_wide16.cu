@@ -31,9 +31,9 @@
 // at the MMA's full rate, at about 2.5 instructions a code; two groups of four
 // warps take alternate stages, so that a group has two stages' time for its
 // chain of loads, conversions, stores and fence.  Warp 18 turns the exponents
-// into 16-bit steps and copies the codes in, some stages ahead of the MMA.  The steps are powers of two, so a code
-// times its step is exact in the operand type and the product is that of the
-// restored matrix.
+// into 16-bit steps and copies the codes in, some stages ahead of the MMA.  The
+// steps are powers of two, so a code times its step is exact in the operand type
+// and the product is that of the restored matrix.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -326,6 +326,14 @@ __global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
         for (int kk = 0; kk < kKB / 16; ++kk)
           umma_bf16_pair(tmem + buf * kTile, desc_a(a0, kk), desc_b(b0, kk), idesc, !fresh || kk != 0);
       };
+      // The converters of both CTAs arrive at the stages of a weight product.
+      auto loaded = [&] {
+        const bool k = MODE == kWideWeight
+                           ? mbar_wait_cluster(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns)
+                           : mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
+        tc_fence_after();
+        return k;
+      };
       auto free_acc = [&](int buf, uint32_t parity) {
         const bool k = mbar_wait(&acce[buf], parity, s_abort, g.status, g.budget_ns);
         tc_fence_after();
@@ -345,9 +353,7 @@ __global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
               if (!(ok = free_acc(buf, ((it >> 1) & 1) ^ 1))) break;
               ++it;
             }
-            ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
-            if (!ok) break;
-            tc_fence_after();
+            if (!(ok = loaded())) break;
             multiply(rg.s, 0, buf, kb == head);
             umma_commit_pair(&empty[rg.s], 0x3);
             rg.next();
@@ -359,9 +365,7 @@ __global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
           if (!(ok = free_acc(0, (it & 1) ^ 1))) break;
           Ring low = rg;
           for (int k = 0; k < first; ++k) {
-            ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
-            if (!ok) break;
-            tc_fence_after();
+            if (!(ok = loaded())) break;
             multiply(rg.s, 0, 0, k == 0);
             rg.next();
           }
@@ -372,9 +376,7 @@ __global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
             low.next();
           }
           for (int kb = kb0 + first; kb < kb1; ++kb) {
-            ok = mbar_wait(&full[rg.s], rg.ph, s_abort, g.status, g.budget_ns);
-            if (!ok) break;
-            tc_fence_after();
+            if (!(ok = loaded())) break;
             multiply(rg.s, 0, 0, false);
             multiply(rg.s, 1, 1, false);
             umma_commit_pair(&empty[rg.s], 0x3);
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(WideCfg<MODE, SUB>::THREADS, 1)
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive_remote(mapa_u32(&full[rg.s], 0));
+          if (lane == 0) mbar_arrive_cluster(mapa_u32(&full[rg.s], 0));
         }
       }
     }
