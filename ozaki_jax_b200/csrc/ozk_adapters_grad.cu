@@ -123,16 +123,26 @@ struct OuterArgs {
   uint64_t budget_ns;
 };
 
+// A word of the row lists.  k_sort_rows may still be writing them when a later
+// kernel of the call starts, so they are read after grid_wait() and by an
+// ordinary load that stays there: __ldg's path wants data that nobody writes
+// while the kernel runs, and its loads may be moved before the wait.
+__device__ __forceinline__ int32_t load_listed(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // The stages of a chunk: up to 64 places [pos, end) of one adapter's rows at a time.
 struct Walk {
   int e, pos, end, first;  // end: of this adapter's rows in the chunk
   __device__ void seek(const int32_t* start, int E, int limit) {
-    while (e < E && __ldg(start + e + 1) <= pos) ++e;
+    while (e < E && load_listed(start + e + 1) <= pos) ++e;
     if (e >= E || pos >= limit) {
       e = E;
       return;
     }
-    const int b = __ldg(start + e + 1);
+    const int b = load_listed(start + e + 1);
     end = b < limit ? b : limit;
     first = pos;
   }
@@ -191,7 +201,7 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
     int lo = 0, hi = g.E - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (__ldg(g.start + mid) <= cur.pos) lo = mid;
+      if (load_listed(g.start + mid) <= cur.pos) lo = mid;
       else hi = mid - 1;
     }
     cur.e = lo;
@@ -203,7 +213,7 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
 #pragma unroll
     for (int i = 0; i < kStep; i += 32) {
       const int p = ahead.pos + i + lane;
-      sh.rows[stage % kRowSlots][i + lane] = ahead.e < g.E && p < ahead.end ? __ldg(g.order + p) : -1;
+      sh.rows[stage % kRowSlots][i + lane] = ahead.e < g.E && p < ahead.end ? load_listed(g.order + p) : -1;
     }
     ahead.next(g.start, g.E, limit);
   };
@@ -351,7 +361,7 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
       done_ph ^= 1;
       if (__syncthreads_or(!ok)) break;
       tc_fence_after();
-      const bool whole = was.first == __ldg(g.start + was.e) && was.end == __ldg(g.start + was.e + 1);
+      const bool whole = was.first == load_listed(g.start + was.e) && was.end == load_listed(g.start + was.e + 1);
       const int mb = (warp >> 2) & 1, q = warp & 3;
       const int64_t c = col0 + mb * 128 + q * 32 + lane;
       const int64_t part = (int64_t)(2 * chunk + (was.first != chunk * g.len)) * g.r * job.C;
@@ -417,7 +427,7 @@ __global__ void __launch_bounds__(kOuterThreads, 1)
   const OuterJob& job = g.job[second];
   const int64_t col0 = (int64_t)((int)blockIdx.x - (second ? g.job[0].tiles : 0)) * kCols;
   const int chunk = blockIdx.y;
-  const int total = __ldg(g.start + g.E);
+  const int total = load_listed(g.start + g.E);
   const int limit = (chunk + 1) * g.len < total ? (chunk + 1) * g.len : total;
   if (chunk * g.len >= limit) return;  // the whole CTA: nothing is allocated yet
   uint32_t cols = 32;
@@ -447,7 +457,7 @@ __global__ void k_outer_join(const __grid_constant__ OuterArgs g) {
   grid_wait();
   const int e = blockIdx.y;
   const OuterJob& job = g.job[blockIdx.z];
-  const int a = __ldg(g.start + e), b = __ldg(g.start + e + 1);
+  const int a = load_listed(g.start + e), b = load_listed(g.start + e + 1);
   const int c0 = a / g.len, c1 = b > a ? (b - 1) / g.len : c0 - 1;
   if (c0 == c1) return;
   const int64_t n = (int64_t)g.r * job.C;

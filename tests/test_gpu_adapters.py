@@ -260,6 +260,24 @@ def test_many_adapters_over_chunks():
     check(Y, want, mY, K + 2 * r + 4, u)
 
 
+def test_row_lists_of_calls_in_a_row():
+    """Calls that nothing waits between, in turn on ids with quite different row lists (the scratch
+    that holds the lists is the same memory each time): every call uses its own lists."""
+    M, N, K, r, E = 3000, 72, 600, 8, 40
+    X, W, A, B, ids, scale, dY = make(M, N, K, r, E, BF16, seed=6)
+    T = torch.randn(M, r, device="cuda")
+    kinds = [ids, torch.full_like(ids, 7), torch.full_like(ids, -1),
+             (torch.arange(M, device="cuda") % E).int(), ids.sort(descending=True).values]
+    want = []
+    for i in kinds:
+        want.append(oz.adapters_grad(dY, X, W, A, B, i, T, scale))
+        torch.cuda.synchronize()
+    got = [oz.adapters_grad(dY, X, W, A, B, i, T, scale)[1:] for _ in range(20) for i in kinds]
+    torch.cuda.synchronize()
+    for j, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[j % len(kinds)][1:]))
+
+
 def test_first_call_of_a_process_may_be_captured():
     """Kernels are loaded and the status word is made inside the capture."""
     import subprocess
