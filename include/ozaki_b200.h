@@ -441,8 +441,9 @@ int ozk_status_word(int32_t** word);
  *   outside [0, E) has no adapter.  scale: FP32 [E] or NULL (ones).
  *   Y [M][N] (ldy) of type dt; low: FP32 [M][r], receives T (0 for rows without
  *   an adapter), or NULL.
- * Sums are FP32; T enters the second product as the sum of two 16-bit values
- * (with OZK_DT_F16, |T| must stay below 65504).  1 <= r <= 128.  Nothing may
+ * Sums are FP32; T enters the second product as the sum of two 16-bit values:
+ * 2^-16 of itself off with OZK_DT_BF16, 2^-22 with OZK_DT_F16, and there also up
+ * to 2^-25 whatever its size; |T| must stay below 65504 there.  1 <= r <= 128.  Nothing may
  * alias Y or low.  Operands whose base or row stride is not a multiple of 16
  * bytes are copied into the workspace first; a workspace asked for with
  * `aligned` set has no room for that. */
@@ -461,7 +462,10 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
  * X: [M][K] (ldx) of type dt, or, with exps set, the int8 codes of
  * ozk_checkpoint_rows made from type dt (ldx = K rounded up to 128).  T: FP32
  * [M][r], the `low` of the forward call.  dX [M][K] (lddx), dA [E][r][K] and
- * dB [E][N][r] of type dt.  Sums over rows are FP32 in a fixed order. */
+ * dB [E][N][r] of type dt.  Sums over rows are FP32 in a fixed order.  With
+ * OZK_DT_F16 U enters dX as T enters Y (off by up to 2^-25), dA and dB take U
+ * and T to 2^-36, and |U| and |T| must stay below 65504.  At most 65535
+ * adapters. */
 size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r, int E,
                                          int aligned);
 int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, const void* exps,

@@ -66,7 +66,9 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
 
     Like the other functions here it records nothing for autograd: the gradients
     are adapters_grad's.  Sums are FP32 and Y is rounded once.  T enters the second product as a sum
-    of two 16-bit values; in float16 |T| must stay below 65504.
+    of two 16-bit values: up to 2^-16 (bfloat16) or 2^-22 (float16) of T off, in float16 also
+    up to 2^-25 whatever T's size, and |T| must stay below 65504 there (a larger one makes its row
+    of Y infinite or NaN).
     """
     (M, Kx), dtype = check_16bit("X", X)
     N, K, E, r, factors, alpha = _adapter_shapes(W, A, B, ids, scale, M, dtype)
@@ -103,6 +105,12 @@ def adapters_grad(dY, X, W, A, B, ids, T, scale=1.0, input_grad=True):
     X is the layer's input (M, K), or its SavedRows.  T is what the forward
     call returned beside Y.  Returns (dX, dA, dB) in the type of dY, dX None
     without input_grad; adapters without rows get zeros.
+
+    U enters dX as T enters Y: in float16 up to 2^-25 off.  dA and dB take U
+    and T to 2^-36 there, so gradients that are small row by row keep their
+    digits.  In float16 |U| and |T| must stay below 65504; beyond, dX of the
+    row, dA and dB of its adapter become infinite or NaN.  At most 65535
+    adapters.  Nothing is recorded for autograd.
     """
     (M, Ny), dtype = check_16bit("dY", dY)
     N, K, E, r, factors, alpha = _adapter_shapes(W, A, B, ids, scale, M, dtype)

@@ -17,9 +17,12 @@
 // NaN, and any order of ids is right; contiguous requests cost one or two
 // chains per tile.
 //
-// T between the kernels.  Rounded once to BF16, T would add an error of 2^-9
-// of itself to every output; as hi + lo it carries 16 bits or more (2^-17), at
-// the price of r more columns of the contraction.
+// T between the kernels.  Rounded once to BF16, T would be up to 2^-8 of itself
+// off; as hi + lo it is 2^-16 (BF16) or 2^-22 (FP16) off, at the price of r more
+// columns of the contraction.  FP16 ends at 2^-24, so there T is also up to 2^-25
+// off whatever its size: with |B| below 1 / sqrt(r) that is less than what Y's
+// own rounding costs.  The sums over rows in dA get a split of U that keeps more
+// (see low_up).
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -313,6 +316,7 @@ struct LowArgs {
   float alpha;
   float* low;        // [M][r] FP32, or NULL
   uint16_t* split;   // [M][2 half], or NULL
+  uint16_t* outer;   // the same with low parts times low_up, or NULL
   int64_t M;
   int nkb, E, r, rp;  // rp: r rounded up to 16
   int batch;          // adapters of a tile that are multiplied at once
@@ -509,14 +513,16 @@ __global__ void __launch_bounds__(kThreads)
       if (c + 2 < g.r) o[2] = t.z;
       if (c + 3 < g.r) o[3] = t.w;
     }
-    if (g.split) {
+    auto store = [&](uint16_t* split, float up) {
       uint32_t hi[2], lo[2];
-      split16(g.bf16, t.x, t.y, hi[0], lo[0]);
-      split16(g.bf16, t.z, t.w, hi[1], lo[1]);
-      uint16_t* o = g.split + row * 2 * half + c;
+      split16(g.bf16, t.x, t.y, up, hi[0], lo[0]);
+      split16(g.bf16, t.z, t.w, up, hi[1], lo[1]);
+      uint16_t* o = split + row * 2 * half + c;
       *(uint2*)o = make_uint2(hi[0], hi[1]);
       *(uint2*)(o + half) = make_uint2(lo[0], lo[1]);
-    }
+    };
+    if (g.split) store(g.split, 1.0f);
+    if (g.outer) store(g.outer, low_up(g.bf16));
   }
   cluster_sync();
   tc_fence_before();
@@ -593,7 +599,7 @@ __global__ void __launch_bounds__(kLowThreads)
       t *= g.scale ? g.alpha * g.scale[i] : g.alpha;
     }
     if (g.low && c < g.r) g.low[row * g.r + c] = t;
-    if (g.split && c < half) store_split(g.split, row, half, c, t, g.bf16);
+    if (g.split && c < half) store_split(g.split, row, half, c, t, g.bf16, 1.0f);
   }
 }
 
@@ -676,13 +682,14 @@ struct Product {
 };
 
 int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float alpha, float* low,
-                 uint16_t* split, int32_t* status, int dev, cudaStream_t stream) {
+                 uint16_t* split, uint16_t* outer, int32_t* status, int dev, cudaStream_t stream) {
   LowArgs g = {};
   g.ids = ids;
   g.scale = scale;
   g.alpha = alpha;
   g.low = low;
   g.split = split;
+  g.outer = outer;
   g.M = p.M;
   g.E = p.E;
   g.r = p.r;
@@ -924,7 +931,9 @@ int ozk_matmul_adapters(const void* X, int64_t ldx, const void* W, int64_t ldw, 
     else if (!workspace || w.used > ws_bytes || ((uintptr_t)workspace & 127))
       return set_error(OZK_ERR_WORKSPACE, "workspace of %zu bytes, aligned to 128, needed", w.used);
   }
-  if ((rc = run_low_rank(p, ids, scale, (float)alpha, low, split, status_dev, dev, s)) || N == 0)
+  if ((rc = run_low_rank(p, ids, scale, (float)alpha, low, split, nullptr, status_dev, dev,
+                         s)) ||
+      N == 0)
     return rc;
   return run_linear(p, ids, split, Y, ldy, status_dev, dev, s);
 }
@@ -935,6 +944,7 @@ size_t ozk_adapters_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int r,
   int dev = 0;
   cudaGetDevice(&dev);
   Arena ws(nullptr);
+  ws.take((size_t)M * 4 * split_half(r));
   ws.take((size_t)M * 4 * split_half(r));
   ws.take(outer_scratch_bytes(M, N, K, r, E, dev));
   if (aligned) return ws.used;
@@ -974,6 +984,8 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   Product p = {{dY, ldy}, {W, ldw}, {B, r}, {A, K}, M, K, N, r, E, true, dt == OZK_DT_BF16};
   Arena ws(workspace);
   uint16_t* split = ws.take<uint16_t>((size_t)M * 4 * split_half(r));
+  // U for dA: in BF16 the same split serves.
+  uint16_t* outer = p.bf16 ? split : ws.take<uint16_t>((size_t)M * 4 * split_half(r));
   void* scratch = ws.take(outer_scratch_bytes(M, N, K, r, E, dev));
   Operand in = {X, ldx};
   for (int pass = 0; pass < 2; ++pass) {
@@ -1002,13 +1014,16 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   o.exps = (const int8_t*)exps;
   o.dY = p.X.p;
   o.ldy = p.X.ld;
-  o.U = split;
+  o.U = outer;
   o.T = T;
   o.dA = dA;
   o.dB = dB;
   o.status = status_dev;
   if ((rc = launch_outer_rows(o, scratch, dev, s))) return rc;
-  if ((rc = run_low_rank(p, ids, scale, (float)alpha, nullptr, split, status_dev, dev, s))) return rc;
+  if ((rc = run_low_rank(p, ids, scale, (float)alpha, nullptr,
+                         p.bf16 || dX ? split : nullptr, p.bf16 ? nullptr : outer, status_dev, dev,
+                         s)))
+    return rc;
   if (dX && (rc = run_linear(p, ids, split, dX, lddx, status_dev, dev, s))) return rc;
   return launch_outer(o, scratch, dev, s);
 }

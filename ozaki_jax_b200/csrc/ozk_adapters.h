@@ -17,7 +17,7 @@ struct OuterProduct {
   const int8_t* exps;
   const void* dY;       // [M][N]
   int64_t ldy;
-  const uint16_t* U;    // [M][2 split_half(r)]: high and low parts
+  const uint16_t* U;    // [M][2 split_half(r)]: high parts, low parts times low_up
   const float* T;       // [M][r]
   void *dA, *dB;        // [E][r][K], [E][N][r]
   int32_t* status;

@@ -12,7 +12,9 @@
 // gathers 64 rows at a time into a ring of shared-memory stages (cp.async, three
 // stages in flight: 96 KB per SM; codes are converted on the way to the tensor
 // cores) and multiplies them: D[256 columns][2 r] += Z^T [hi | lo], the halves
-// being added at the end.  One warp issues the MMAs (about 90 clocks each at
+// being added at the end (in FP16 lo is held 2^11 times as large, so that U and
+// T count to 2^-36 however small they are; rows of a gradient of 1e-7 add up to
+// values that FP16 holds).  One warp issues the MMAs (about 90 clocks each at
 // these widths, bound by reading Z from shared memory) and one looks the next
 // rows up, beside the sixteen that fetch: with the issue and the lookup in the
 // fetching warps a stage took 5400 clocks.  Rows of other
@@ -56,7 +58,7 @@ __global__ void __launch_bounds__(kSortThreads)
          i += (int64_t)((int)gridDim.x - E) * kSortThreads) {
       const int64_t m = i / half;
       const int c = (int)(i - m * half);
-      store_split(split, m, half, c, c < r ? T[m * r + c] : 0.0f, bf16);
+      store_split(split, m, half, c, c < r ? T[m * r + c] : 0.0f, bf16, low_up(bf16));
     }
     return;
   }
@@ -103,7 +105,7 @@ struct OuterJob {
   const void* Z;         // 16-bit [M][C], or int8 codes when exps is set
   int64_t ldz, C;
   const int8_t* exps;    // [groups][M]
-  const uint16_t* L;     // [M][2 split_half(r)]: high parts, low parts
+  const uint16_t* L;     // [M][2 split_half(r)]: high parts, low parts times low_up
   float* partial;        // [2 chunks][r C], see below
   void* out;             // [E][r][C], or [E][C][r] when trans
   int trans, tiles;
@@ -375,7 +377,8 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
         if (c >= job.C) continue;
         float sum[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) sum[k] = __uint_as_float(v[k]) + __uint_as_float(w[k]);
+        for (int k = 0; k < 16; ++k)
+          sum[k] = fmaf(__uint_as_float(w[k]), low_down(BF16), __uint_as_float(v[k]));
         if (job.trans && (g.r & 7) == 0) {
           // a thread's ranks lie side by side: 8 at a time
 #pragma unroll

@@ -144,23 +144,31 @@ __device__ __forceinline__ void ring_drain(uint64_t* full, int stages, int steps
 // ceil(r / 64) blocks of 64.
 __host__ __device__ inline int split_half(int r) { return r <= 32 ? 32 : (r + 63) / 64 * 64; }
 
-// Two FP32 values as high and low 16-bit parts, packed.
-__device__ __forceinline__ void split16(bool bf16, float a, float b, uint32_t& hi, uint32_t& lo) {
+// Low parts that a product of their own multiplies are held 2^11 times as large
+// in FP16, whose smallest number is 2^-24: the value is then held to 2^-36
+// instead of 2^-25.  (What rounding to FP16 leaves of a value below 65520 is at most 16, so
+// nothing overflows.)  BF16 has FP32's range.
+__host__ __device__ constexpr float low_up(bool bf16) { return bf16 ? 1.0f : 2048.0f; }
+__host__ __device__ constexpr float low_down(bool bf16) { return bf16 ? 1.0f : 1.0f / 2048.0f; }
+
+// Two FP32 values as high and low 16-bit parts, packed; `up`: what the low
+// parts are multiplied by, a power of two.
+__device__ __forceinline__ void split16(bool bf16, float a, float b, float up, uint32_t& hi,
+                                        uint32_t& lo) {
   hi = pack16(bf16, a, b);
   float ra = a - widen16(bf16, (uint16_t)hi), rb = b - widen16(bf16, (uint16_t)(hi >> 16));
   if (!(fabsf(ra) <= 3.0e38f)) ra = 0.0f;  // not finite: the high part says so by itself
   if (!(fabsf(rb) <= 3.0e38f)) rb = 0.0f;
-  lo = pack16(bf16, ra, rb);
+  lo = pack16(bf16, ra * up, rb * up);
 }
 
 // Rounds t to its high and low 16-bit parts and stores them in the split T.
 __device__ __forceinline__ void store_split(uint16_t* split, int64_t row, int half, int c, float t,
-                                            bool bf16) {
-  const uint16_t hi = round16(bf16, t);
-  float rest = t - widen16(bf16, hi);
-  if (!(fabsf(rest) <= 3.0e38f)) rest = 0.0f;  // t not finite: hi says so by itself
-  split[row * 2 * half + c] = hi;
-  split[row * 2 * half + half + c] = round16(bf16, rest);
+                                            bool bf16, float up) {
+  uint32_t hi, lo;
+  split16(bf16, t, 0.0f, up, hi, lo);
+  split[row * 2 * half + c] = (uint16_t)hi;
+  split[row * 2 * half + half + c] = (uint16_t)lo;
 }
 
 // ------------------------------------------------- int8 checkpoint codes

@@ -128,6 +128,49 @@ def test_grads(case, dt, saved):
     assert none is None and torch.equal(dA, got[1]) and torch.equal(dB, got[2])
 
 
+@pytest.mark.parametrize("dy, b", [(1e-1, 1e-5), (1e-4, 1e-3), (1e-4, 1e-4), (2e-5, 1e-4)])
+@pytest.mark.parametrize("saved", [False, True])
+def test_small_float16_gradients(dy, b, saved):
+    """Gradients of ordinary float16 training: U (and T) far below 2^-14, dA and dB of rows enough
+    to be held.  U and T are held to 2^-22 of themselves (two roundings of 2^-11) and to 2^-36, so
+    dA is off by that share of the magnitudes and 2^-36 of the sum of |X|, by the FP32 sums, and by
+    its own rounding: 2^-11 of itself or half of float16's smallest number, 2^-25."""
+    M, N, K, r, E = 4096, 512, 256, 16, 2
+    X, W, A, B, ids, scale, dY = make(M, N, K, r, E, F16, seed=8)
+    dY, B = (dY.float() * (10 * dy)).half(), (B.float() * b).half()
+    T = (1e-6 * torch.randn(M, r, generator=torch.Generator(device="cuda").manual_seed(5),
+                            device="cuda"))
+    S = oz.checkpoint_rows(X) if saved else X
+    X64 = (oz.restore_rows(S) if saved else X).double()
+    got = oz.adapters_grad(dY, S, W, A, B, ids, T, scale)
+    want, size = grads64(dY, X64, W, A, B, ids, T, scale)
+    u, low = 2.0 ** -11, 2.0 ** -25
+    for name, k, terms, other in (("dA", 1, M + N + 4, X64.abs()), ("dB", 2, M + 4, dY.double().abs())):
+        mag = torch.zeros_like(want[k])
+        for i, rows in rows_of(ids, E):
+            s = other[rows].sum(0)
+            mag[i] = s[None, :] if k == 1 else s[:, None]
+        err = (got[k].double() - want[k]).abs()
+        bound = (u * want[k].abs()).clamp(min=low) + (1 + u) * (
+            (terms * STEP + 2.0 ** -21) * size[k] + 2.0 ** -36 * mag)
+        assert bool((err <= bound).all()), (name, float((err / bound).max()))
+        # as a whole: the rounding, at most `low` or u of each value, and little else
+        room = (u * want[k].abs()).clamp(min=low).norm() + 2.0 ** -36 * mag.norm()
+        assert float(err.norm()) <= 1.01 * float(room) + 1e-5 * float(want[k].norm())
+
+
+def test_large_float16_rows_of_t():
+    """T and U up to float16's limit: finite where the definition is."""
+    M, N, K, r, E = 300, 64, 96, 8, 2
+    X, W, A, B, ids, scale, dY = make(M, N, K, r, E, F16, seed=8)
+    dY = (dY.float() * 2 ** -10).half()
+    T = 65503.0 * torch.sign(torch.randn(M, r, device="cuda"))
+    T[::3] = 65488.0  # a tie of FP16's rounding: the low part is the largest there is
+    got = oz.adapters_grad(dY, X, W, A, B, ids, T, scale)
+    want, size = grads64(dY, X, W, A, B, ids, T, scale)
+    check(got[2], want[2], size[2], M + 4, 2.0 ** -11)
+
+
 def test_gradients_against_differences():
     """<dL/dp, d> = (L(p + d) - L(p - d)) / 2 for L = <dY, Y>, which is linear in each of X, A, B."""
     M, N, K, r, E = 150, 96, 80, 8, 3
