@@ -319,16 +319,30 @@ inline size_t tmem_share(int cols) {
   return (size_t)c * 432;
 }
 
-// Lets kernel K use `bytes` of dynamic shared memory on device dev; the driver
-// is asked once per size that is larger than those before.
+// Lets kernel K use `bytes` of dynamic shared memory on device dev.  The limit
+// is an attribute of the kernel that a call sets, not raises: so it is set once,
+// to all that the device gives a CTA besides K's static shared memory, and
+// threads whose calls need different sizes cannot lower it under each other.
+// (A launch's own size, not the limit, decides how many CTAs fit an SM.)
 template <auto K>
 int allow_smem(size_t bytes, int dev) {
   static std::atomic<int> allowed[64];
   if (dev < 0 || dev >= 64) return set_error(OZK_ERR_ARG, "device %d", dev);
-  if ((int)bytes <= allowed[dev].load(std::memory_order_relaxed)) return OZK_OK;
-  cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute", e);
-  allowed[dev].store((int)bytes, std::memory_order_relaxed);
+  int most = allowed[dev].load(std::memory_order_acquire);
+  if (!most) {
+    cudaFuncAttributes a;
+    cudaError_t e = cudaFuncGetAttributes(&a, K);
+    if (e == cudaSuccess)
+      e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+    if (e == cudaSuccess) {
+      most -= (int)a.sharedSizeBytes;
+      e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    }
+    if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute", e);
+    allowed[dev].store(most, std::memory_order_release);
+  }
+  if (bytes > (size_t)most)
+    return set_error(OZK_ERR_UNSUPPORTED, "%zu bytes of shared memory needed, %d there", bytes, most);
   return OZK_OK;
 }
 

@@ -348,6 +348,52 @@ def test_first_call_of_a_process_may_be_captured():
     assert p.returncode == 0 and "captured" in p.stdout, p.stderr[-2000:]
 
 
+def test_first_calls_of_two_threads():
+    """Two threads of a fresh process call at the same moments with shapes whose kernels need
+    different sizes of shared memory, growing from step to step: no call may fail, and each result
+    is the one that a thread alone gets."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    code = (
+        "import sys, threading, torch, ozaki_jax_b200 as oz\n"
+        "sys.setswitchinterval(1e-6)\n"
+        "def data(M, r):\n"
+        "    g = torch.Generator(device='cuda').manual_seed(1000 * r + M)\n"
+        "    f = lambda *s: torch.randn(*s, generator=g, device='cuda').bfloat16()\n"
+        "    ids = torch.randint(0, 2, (M,), generator=g, device='cuda', dtype=torch.int32)\n"
+        "    return f(M, 64), f(72, 64), f(2, r, 64), f(2, 72, r), ids, f(M, 72), f(M, r).float()\n"
+        "def call(X, W, A, B, ids, dY, T):\n"
+        "    return (oz.matmul_adapters(X, W, A, B, ids),\n"
+        "            *oz.adapters_grad(dY, X, W, A, B, ids, T))\n"
+        "shapes = [[(M, r) for r in (8, 40, 56, 72, 104, 120) for M in range(8 + 8 * t, 200, 16)]\n"
+        "          for t in (0, 1)]\n"
+        "sets = [[data(*s) for s in list_] for list_ in shapes]\n"
+        "torch.cuda.synchronize()\n"
+        "start, got, failed = threading.Barrier(2), [[], []], []\n"
+        "def walk(t):\n"
+        "    with torch.cuda.stream(torch.cuda.Stream()):\n"
+        "        for s in sets[t]:\n"
+        "            start.wait(60)\n"
+        "            try:\n"
+        "                got[t].append(call(*s))\n"
+        "            except Exception as e:\n"
+        "                failed.append(repr(e))\n"
+        "                got[t].append(None)\n"
+        "        torch.cuda.current_stream().synchronize()\n"
+        "threads = [threading.Thread(target=walk, args=(t,)) for t in (0, 1)]\n"
+        "[t.start() for t in threads]; [t.join() for t in threads]\n"
+        "assert not failed, failed\n"
+        "for t in (0, 1):\n"
+        "    for a, s in zip(got[t], sets[t]):\n"
+        "        assert all(torch.equal(x, y) for x, y in zip(a, call(*s)))\n"
+        "print('both')\n")
+    p = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True,
+                       timeout=120)
+    assert p.returncode == 0 and "both" in p.stdout, p.stderr[-2000:]
+
+
 def test_streams_and_graphs():
     """Two calls at once on two streams, and a captured call replayed on other data."""
     M, N, K, r, E = 40, 256, 320, 16, 8
