@@ -501,10 +501,15 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t row = row0 + r;
     float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const int i = row_adapter(g.ids, row, g.M, g.E);
-    if (i >= 0 && c < g.r) {  // (columns r to rp of the sums are zero)
+    if (i >= 0 && c < g.r) {
       t = cluster_sum4(smem_u32(&part[r * ldp + c]), (int)splits);
       const float f = g.scale ? g.alpha * g.scale[i] : g.alpha;
       t.x *= f, t.y *= f, t.z *= f, t.w *= f;
+      // Beyond rank r the adapter read as zeros, but an infinity in the row has
+      // made NaNs of them.
+      if (c + 1 >= g.r) t.y = 0.0f;
+      if (c + 2 >= g.r) t.z = 0.0f;
+      if (c + 3 >= g.r) t.w = 0.0f;
     }
     if (g.low) {
       float* o = g.low + row * g.r + c;

@@ -228,6 +228,27 @@ def test_rows_of_no_adapter_and_foreign_nans(M):
         assert not bool(dA[others].isnan().any())
 
 
+@pytest.mark.parametrize("r", [1, 5, 6, 7, 8, 33, 66, 127])
+@pytest.mark.parametrize("M", [20, 200, 2600])
+def test_infinities_of_a_row(M, r):
+    """An infinity in a row of X (or dY) whose products all have one sign makes its row of T, Y (or
+    dX) infinite, not NaN, at every rank and number of rows; the other rows keep their bits."""
+    N, K, E = 2600 if M > 1000 else 72, 136, 2
+    X, W, A, B, ids, scale, dY = (t.abs() if t.is_floating_point() else t
+                                  for t in make(M, N, K, r, E, BF16, seed=2))
+    ids[0], ids[1] = 1, 0
+    T = torch.ones(M, r, device="cuda")
+    X2, dY2 = X.clone(), dY.clone()
+    X2[0, 3] = dY2[0, 3] = float("inf")
+    Y, low = oz.matmul_adapters(X2, W, A, B, ids, scale, return_low=True)
+    clean = oz.matmul_adapters(X, W, A, B, ids, scale)
+    assert bool((low[0] == float("inf")).all()) and bool((Y[0] == float("inf")).all())
+    assert torch.equal(Y[1:], clean[1:])
+    dX = oz.adapters_grad(dY2, X, W, A, B, ids, T, scale)[0]
+    assert bool((dX[0] == float("inf")).all())
+    assert torch.equal(dX[1:], oz.adapters_grad(dY, X, W, A, B, ids, T, scale)[0][1:])
+
+
 def test_adapters_without_rows_and_one_adapter():
     X, W, A, B, ids, scale, dY = make(50, 40, 64, 8, 6, BF16)
     ids[:] = 4
