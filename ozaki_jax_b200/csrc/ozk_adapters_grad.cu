@@ -27,6 +27,7 @@
 // result does not depend on scheduling.
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -377,8 +378,12 @@ __device__ void outer_body(const OuterArgs& g, const OuterJob& job, int64_t col0
         if (c >= job.C) continue;
         float sum[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          sum[k] = fmaf(__uint_as_float(w[k]), low_down(BF16), __uint_as_float(v[k]));
+        for (int k = 0; k < 16; ++k) {
+          // An infinity says so in the high parts' sum; times a low part that is
+          // zero or of the other sign it would become a NaN.
+          const float h = __uint_as_float(v[k]);
+          sum[k] = fabsf(h) < INFINITY ? fmaf(__uint_as_float(w[k]), low_down(BF16), h) : h;
+        }
         if (job.trans && (g.r & 7) == 0) {
           // a thread's ranks lie side by side: 8 at a time
 #pragma unroll

@@ -249,6 +249,33 @@ def test_infinities_of_a_row(M, r):
     assert torch.equal(dX[1:], oz.adapters_grad(dY, X, W, A, B, ids, T, scale)[0][1:])
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_infinities_in_the_gradients_sums(dt):
+    """dA and dB of an infinity whose products all have one sign are infinite, not NaN, though U and
+    T are multiplied in two parts of which one may be zero or negative."""
+    M, N, K, r, E = 300, 72, 136, 8, 3
+    X, W, A, B, ids, scale, dY = (t.abs() if t.is_floating_point() else t
+                                  for t in make(M, N, K, r, E, dt, seed=2))
+    B[1, :, 0] = 0.0
+    B[1, 7, 0] = 1.0   # U's first column is dY's column 7 times the scale: no low part
+    scale[1] = 1.0
+    ids[0], ids[1] = 1, 0
+    T = torch.rand(M, r, device="cuda") + 0.01
+    T[0, 0] = 0.5
+    ref = oz.adapters_grad(dY, X, W, A, B, ids, T, scale)
+    X2, dY2 = X.clone(), dY.clone()
+    X2[0, 3] = float("inf")
+    dA = oz.adapters_grad(dY, X2, W, A, B, ids, T, scale)[1]
+    assert bool((dA[1, :, 3] == float("inf")).all())
+    dA[1, :, 3] = ref[1][1, :, 3]
+    assert torch.equal(dA, ref[1])
+    dY2[0, 5] = float("inf")
+    dB = oz.adapters_grad(dY2, X, W, A, B, ids, T, scale)[2]
+    assert bool((dB[1, 5] == float("inf")).all())
+    dB[1, 5] = ref[2][1, 5]
+    assert torch.equal(dB, ref[2])
+
+
 def test_adapters_without_rows_and_one_adapter():
     X, W, A, B, ids, scale, dY = make(50, 40, 64, 8, 6, BF16)
     ids[:] = 4
