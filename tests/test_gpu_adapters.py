@@ -128,6 +128,31 @@ def test_grads(case, dt, saved):
     assert none is None and torch.equal(dA, got[1]) and torch.equal(dB, got[2])
 
 
+# More 256 x 256 tiles than CTA pairs, so that a pair takes several: with single and with double
+# tiles, all ring places used more than once, the lists of adapters replaced from tile to tile.
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("case, order", [
+    ((200, 19301, 64, 8, 5), "random"),      # one row of tiles: single ones, odd width
+    ((5000, 2600, 130, 40, 4), "sorted"),    # 220 single tiles
+    ((5120, 5120, 320, 16, 3), "sorted"),    # 200 double tiles
+    ((5200, 5208, 448, 100, 40), "random"),  # 210 double tiles, many adapters in each
+])
+def test_forward_of_many_tiles(case, order, dt):
+    test_forward(case, dt, order)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("case, saved", [
+    ((200, 64, 19304, 16, 2), False),   # dX: one row of tiles
+    ((2600, 96, 2500, 8, 5), True),     # 60 double tiles
+    ((5000, 320, 2600, 16, 3), False),  # 220 single tiles
+    ((5200, 450, 5200, 72, 6), True),   # 210 double tiles
+    ((5120, 320, 5127, 100, 40), False),
+])
+def test_grads_of_many_tiles(case, saved, dt):
+    test_grads(case, dt, saved)
+
+
 @pytest.mark.parametrize("dy, b", [(1e-1, 1e-5), (1e-4, 1e-3), (1e-4, 1e-4), (2e-5, 1e-4)])
 @pytest.mark.parametrize("saved", [False, True])
 def test_small_float16_gradients(dy, b, saved):

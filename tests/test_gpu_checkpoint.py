@@ -131,6 +131,19 @@ def test_weight_gradient(case, dt):
                      + 1e-30).all())
 
 
+# More output tiles than CTA pairs, contractions longer than a ring and than one accumulation.
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("case", [
+    (1100, 2600, 2000),  # FP32: two accumulations of a tile, added in the output
+    (9000, 600, 600),    # eight parts, each of two accumulations
+    (700, 5120, 5120),   # 16 bits: 200 double tiles
+    (300, 5000, 2601),   # 220 single tiles, odd width
+    (2100, 5100, 2600),  # FP32: three accumulations, several tiles of a CTA pair
+])
+def test_weight_gradient_of_many_tiles(case, dt):
+    test_weight_gradient(case, dt)
+
+
 def test_weight_gradient_of_nan_groups():
     """A group that held a NaN makes its 128 columns NaN and no others; rows that do not exist add
     nothing."""
