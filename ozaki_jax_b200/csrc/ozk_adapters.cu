@@ -970,6 +970,7 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   if (rc) return rc;
   if (E > 65535) return set_error(OZK_ERR_UNSUPPORTED, "at most 65535 adapters");
   if (!dA || (N && !dB)) return set_error(OZK_ERR_ARG, "NULL dA or dB");
+  if (dX && lddx < K) return set_error(OZK_ERR_ARG, "lddx < K");
   cudaStream_t s = (cudaStream_t)stream;
   if (M == 0 || N == 0) {
     // No rows or no outputs: the gradients are zero.
@@ -983,7 +984,6 @@ int ozk_adapters_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, c
   if (exps ? (ldx != round_up(K, kGroup) || ((uintptr_t)X & 15)) : ldx < K)
     return set_error(OZK_ERR_ARG, exps ? "codes need 16 bytes of alignment and ldx = K rounded up to 128"
                                        : "ldx < K");
-  if (dX && lddx < K) return set_error(OZK_ERR_ARG, "lddx < K");
   int dev;
   cudaGetDevice(&dev);
   Product p = {{dY, ldy}, {W, ldw}, {B, r}, {A, K}, M, K, N, r, E, true, dt == OZK_DT_BF16};

@@ -100,6 +100,16 @@ def test_checkpoint_refusals():
         oz.checkpoint_grad(z(3, 5), s)
 
 
+def test_grad_without_outputs_refuses_a_short_row_of_dx():
+    """N = 0: dX is only zeroed, with rows of lddx elements all the same."""
+    from ozaki_jax_b200 import _lib
+    lib = _lib.load()
+    p = 1 << 20  # never dereferenced here
+    assert lib.ozk_adapters_grad(p, 0, p, 16, None, p, 16, p, p, p, p, None, 1.0, p, 15, p, p, 4, 0,
+                                 16, 4, 2, 0, None, 0, None, None) == _lib.OZK_ERR_ARG
+    assert "lddx" in _lib.detail()
+
+
 def test_entry_points_refuse_before_device_work():
     from ozaki_jax_b200 import _lib
     lib = _lib.load()
