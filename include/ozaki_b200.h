@@ -489,8 +489,11 @@ int ozk_restore_rows(const void* codes, int64_t ldc, const void* exps, int64_t M
                      void* out, int64_t ldo, int dt, void* stream);
 /* Weight gradient from a checkpointed input: out = dY^T X^ (+ out with
  * accumulate), dY [M][N] (ldy, type dt: OZK_DT_BF16 or OZK_DT_F16), X^ [M][K]
- * the restored rows, out [N][K] (ldo) of type out_dt (dt or OZK_DT_F32).  FP32
- * sums, one rounding.  The result does not depend on scheduling: where the
+ * the restored rows, out [N][K] (ldo) of type out_dt (dt or OZK_DT_F32), which
+ * overlaps no input.  FP32 sums, one rounding; those of a 16-bit result are
+ * 1.7e-5 off after 16384 rows, in proportion to the rows (the tensor cores cut
+ * off instead of rounding), those of an FP32 result are taken over every 1024
+ * rows.  The result does not depend on scheduling: where the
  * rows are split, the parts are added in order. */
 size_t ozk_checkpoint_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int aligned);
 int ozk_checkpoint_grad(const void* dY, int64_t ldy, const void* codes, int64_t ldc,

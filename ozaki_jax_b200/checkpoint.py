@@ -66,7 +66,8 @@ class SavedRows:
 
 def checkpoint_rows(X):
     """The rows of a CUDA tensor X (M, K), bfloat16, float16 or float32, as
-    SavedRows: about half the bytes of a 16-bit X, a quarter of a float32 one."""
+    SavedRows: about half the bytes of a 16-bit X, a quarter of a float32 one.
+    At most 2097120 rows.  Nothing is recorded for autograd."""
     M, K = check_matrix("X", X)
     dtype = X.dtype
     if dtype not in DTYPES:
@@ -111,8 +112,15 @@ def checkpoint_grad(dY, saved, out=None, accumulate=False, dtype=None):
 
     dY (M, N): bfloat16 or float16, the type that `saved` was made from.  The
     result (N, K) is of that type or, with dtype, float32; it goes to `out`
-    if given (its rows may be strided), and with accumulate it is added to
-    what `out` holds.  FP32 sums, rounded once.
+    if given (its rows may be strided; it may overlap no input), and with
+    accumulate it is added to what `out` holds.  FP32 sums, rounded once.
+    Nothing is recorded for autograd.
+
+    A float32 result is summed in chains of 1024 rows; a 16-bit one in a single
+    chain of the tensor cores, which cut off instead of rounding: 1.7e-5 off after
+    16384 rows, before its own rounding, and in proportion to the rows.  What the call saves is the restored matrix's
+    memory: where there is room for that, dY.T @ restore_rows(saved) takes
+    less time.
     """
     (M, N), dtype_y = check_16bit("dY", dY)
     if not isinstance(saved, SavedRows):

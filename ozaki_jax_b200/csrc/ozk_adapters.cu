@@ -78,9 +78,9 @@ __device__ __forceinline__ float4 cluster_sum4(uint32_t a, int splits) {
 
 // ---------------------------------------------------------------- k_linear
 //
-// Few rows: bound by reading W once (one row of 4096 x 4096: the call takes 11 us
-// in a graph, of which W's 33.5 MB need 5.1; 64 rows of 8192 x 4096 with 64
-// adapters: 20 us, 12.9 by their bytes).  The tokens are the MMA's M side even
+// Few rows: bound by reading W once (one row of 4096 x 4096: the call takes 12 to
+// 17 us in a graph, of which W's 33.5 MB need 5.1; 64 rows of 8192 x 4096 with 64
+// adapters: 25 to 29 us, 12.9 by their bytes).  The tokens are the MMA's M side even
 // then: 128 lanes of which few are used cost N / 2 clocks per 16 indexes, less
 // than the 1.4 N that W's bytes take from memory.
 // One CTA per 128 x BN tile, or a cluster of CTAs per tile that split the
@@ -722,7 +722,8 @@ int run_low_rank(const Product& p, const int32_t* ids, const float* scale, float
   const int64_t tiles = (p.M + kRows - 1) / kRows;
   // Two CTAs per SM at most (a second wave doubles the time), clusters of four
   // where there are tiles enough (of eight, only 15 fit the GPU at 100 KB of
-  // shared memory a CTA), and chains of at most 512 elements.
+  // shared memory a CTA), and chains of at most 512 elements up to a contraction of
+  // 16384 (8192 from rank 65 on; beyond, they grow with it).
   int splits = 1;
   while (splits < (tiles <= 8 ? 8 : 4) && tiles * splits * 2 <= 2 * device_sm_count(dev) &&
          g.nkb >= splits * 4)
@@ -842,8 +843,8 @@ int run_linear(const Product& p, const int32_t* ids, const uint16_t* split, void
     return launch_wide(w, dev, stream);
   }
   // 128 columns per CTA; the contraction split over a cluster as long as two
-  // CTAs per SM hold them all (a second wave doubles the time: 64 x 8192 x 4096
-  // took 20 us with 256 CTAs and 30 us with 512).  Full tiles have more to add
+  // CTAs per SM hold them all (a second wave adds half: 64 x 8192 x 4096, its
+  // inputs in the L2 cache, took 20 us with 256 CTAs and 30 us with 512).  Full tiles have more to add
   // up: they are split in four at most, into parts of sixteen stages or more
   // (1023 x 2048 x 1000 took 17 us whole and 22 us halved, 1777 x 1001 x 2000
   // 37 us whole and 24 us halved).

@@ -6,18 +6,20 @@
 //
 // Persistent: each CTA pair (cta_group::2, M = 256) walks its tiles; each CTA
 // stages its 128 rows of A and half of B's 256 columns per 64 contraction
-// indexes.  Bound by shared memory: a stage of 4 MMAs lasts 512 clocks on the
-// tensor cores, in which the MMAs read 32 KB of each SM's shared memory and
-// the copies write 32 KB; that is all of its 128 B/clk, and a stage took 714
-// clocks (859 with the converters' traffic).  So where there are tiles enough,
+// indexes.  Bound by shared memory, by this count: a stage of 4 MMAs lasts 512
+// clocks on the tensor cores, in which the MMAs read 32 KB of each SM's shared
+// memory and the copies write 32 KB; that is all of its 128 B/clk, and a stage
+// took 714 clocks (859 with the converters' traffic).  So where there are tiles enough,
 // a pair takes two tiles one below the other (SUB = 2, 512 x 256) that share
 // B: 112 KB instead of 128 KB for the same work, and in the weight product
 // each code is converted for 512 rows instead of 256.
 //
-// 16384 x 8192 x 8192 from codes: 1.36 to 1.65 ms by the power limit (1.35 to
-// 1.6 PFLOP/s, 76 to 92% of cuBLAS's BF16 product of the restored matrix),
-// 1.82 ms with SUB = 1.  8192 x 8192 x 4096 with a rank of 64: 375 us (1.47
-// PFLOP/s; cuBLAS without the adapters 345 us).
+// 16384 x 8192 x 8192 from codes: 1.63 ms in a burst and 1.88 ms under the power
+// limit (1.35 and 1.17 PFLOP/s; restoring the rows and cuBLAS's BF16 product
+// 1.33 and 1.56 ms in the same runs).  To FP32, with SUB = 1 and every chain's
+// sums added in the output, 3.74 ms.  8192 x 8192 x 4096 with a rank of 64, the
+// whole call: 388 us in a burst, 456 us under the power limit (cuBLAS without
+// the adapters 408 us there).
 //
 // SUB = 1: two TMEM accumulators (all 512 columns) let the epilogue of one tile
 // run under the MMAs of the next.  SUB = 2: they belong to the two halves of a
@@ -719,7 +721,8 @@ int launch_wide(const WideProduct& p, int dev, cudaStream_t stream) {
   // The tensor cores cut off what a sum's exponent leaves no room for, so an
   // error grows with the length of the chain: an FP32 result was 1.7e-5 off
   // after 16384 FP16 rows, 7e-7 after 1024.  FP32 results are summed in chains
-  // of 1024; a 16-bit rounding hides it.
+  // of 1024.  16-bit results are not: 1.7e-5 changes 0.13% of the BF16 values of a
+  // sum of 16384, each by one step.
   g.chain = p.out_f32 || g.splits > 1 ? 16 : 1 << 30;
   g.bf16 = p.bf16;
   g.out_f32 = p.out_f32;
