@@ -68,7 +68,8 @@ def matmul_adapters(X, W, A, B, ids=None, scale=1.0, return_low=False):
     are adapters_grad's.  Sums are FP32 and Y is rounded once.  T enters the second product as a sum
     of two 16-bit values: up to 2^-16 (bfloat16) or 2^-22 (float16) of T off, in float16 also
     up to 2^-25 whatever T's size, and |T| must stay below 65504 there (a larger one makes its row
-    of Y infinite or NaN).
+    of Y infinite or NaN). An infinity in B may come out as a NaN, the parts' products
+    having different signs.
     """
     (M, Kx), dtype = check_16bit("X", X)
     N, K, E, r, factors, alpha = _adapter_shapes(W, A, B, ids, scale, M, dtype)
